@@ -229,7 +229,7 @@ def _own(s):
         else:
             s.call = (_backend.logits_adjust, ku.LogitsArgs(
                 dtype=types_[c.dtype], out_dtype=types_[c.out], rows=c.rows, vocab=c.vocab, logits=p(s.logits), logits_stride=s.logits.stride(0),
-                out=p(s.out), out_stride=s.out.stride(0), tokens=p(s.tokens), tokens_stride=s.tokens.stride(0), lens=p(s.lengths),
+                out=p(s.out), out_stride=s.out.stride(0), history=c.history, tokens=p(s.tokens), tokens_stride=s.tokens.stride(0), lens=p(s.lengths),
                 prompt_lens=p(s.prompt), repetition=p(s.repetition), presence=p(s.presence), frequency=p(s.frequency),
                 bias_ids=p(s.bias_ids), bias_values=p(s.bias_values), bias_offsets=p(s.bias_offsets), bias_count=s.bias_ids.numel(), mask=p(s.mask),
                 mask_rows=s.mask.shape[0], mask_stride=s.mask.stride(0), mask_index=p(s.mask_rows)))
