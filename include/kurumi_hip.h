@@ -292,6 +292,172 @@ int32_t ku_hip_linear_e4m3(const KuBackend *b, const void *x, uint32_t x_dtype, 
 int32_t ku_hip_linear_e4m3_noalloc(const void *x, uint32_t x_dtype, const uint8_t *wq, const float *sw, void *y,
                                    uint32_t y_dtype, size_t m, size_t n, size_t k, void *stream);
 
+/* ---- one decode step on caller-owned device buffers ----
+ *
+ * What a program that generates several answers to one prompt needs around the graph's rope, sdpa
+ * and softmax / argmax: rotary positions that are data, stored into a key / value cache that is
+ * written in place; attention that reads the prompt's keys and values once for the whole batch; and
+ * the adjustment of the logits. No counterpart in the reference, whose IR is functional (a cache
+ * cannot be written in place, lengths are shapes).
+ *
+ * Each call takes one block of arguments: clear it, set `size` to sizeof the struct and what the call
+ * needs. Pointers are device memory of the backend's GPU unless said otherwise, strides are in
+ * elements, dtypes are KU_F32, KU_BF16 or KU_F16. The call is enqueued on `stream` (a hipStream_t;
+ * NULL = the backend's stream) asynchronously, and reads the block (and `freqs`) before it returns,
+ * so both may be reused at once. It leaves the current device as it was. Returns 0, or -1 with
+ * ku_last_error; a refused call has launched nothing. Values that only the device sees (positions,
+ * lengths, indices) are bounds-checked there as each field says; they never make a kernel read or
+ * write outside the buffers that the block describes. All three may be captured into a hipGraph. */
+
+typedef enum { KU_ROPE_HALF = 0, KU_ROPE_INTERLEAVED = 1 } KuRopeLayout;
+typedef enum { KU_ROPE_UNSCALED = 0, KU_ROPE_LINEAR, KU_ROPE_BASE, KU_ROPE_BY_PARTS } KuRopeScaling;
+
+/* Angular frequencies (radians a position) of rot_dim / 2 rotary pairs into out (host memory):
+ * f_i = base^(-2i / rot_dim), for contexts longer than the trained one as
+ *   KU_ROPE_LINEAR   f_i / factor (positions interpolated)
+ *   KU_ROPE_BASE     base times factor^(rot_dim / (rot_dim - 2)): the fastest pair keeps its
+ *                    frequency, the slowest is divided by factor
+ *   KU_ROPE_BY_PARTS pairs that turn at least `high` times over `trained_len` positions keep their
+ *                    frequency, those that turn at most `low` times are divided by factor, and those
+ *                    between are blended linearly in the number of turns
+ * `trained_len`, `low` and `high` count for KU_ROPE_BY_PARTS only. Returns 0, or -1 with
+ * ku_last_error. Needs no GPU. */
+int32_t ku_hip_rope_freqs(size_t rot_dim, double base, uint32_t scaling, double factor, double trained_len, double low,
+                          double high, double *out);
+
+/* ku_hip_rope: y = scale * R(position) x on the first rot_dim features of every head, the others
+ * copied. Pair i of a head is features (i, i + rot_dim / 2) for KU_ROPE_HALF and (2i, 2i + 1) for
+ * KU_ROPE_INTERLEAVED; its angle is position * freqs[i], formed in 64 bits. `inverse` != 0 turns by
+ * the negative angles: the transpose of the forward map, and so its gradient.
+ *   q [tokens, q_heads, head_dim] -> q_out of that shape
+ *   k [tokens, kv_heads, head_dim], rotated -> row rows[t] of k_out [out_rows, kv_heads, head_dim]
+ *   v [tokens, kv_heads, head_dim], copied  -> row rows[t] of v_out
+ * q, k and v are each optional (NULL with a NULL output). rows NULL: token t goes to row t. A token
+ * whose row is outside [0, out_rows) is not stored (a padded batch: -1); rows that no token names
+ * keep what they hold. Rows of one call have to differ: of two tokens with one row, either's values
+ * may stay. An output may be its input itself (same pointer and strides; k and v then without
+ * rows), otherwise they may not overlap. Any strides and alignments; where heads, strides and
+ * pointers are multiples of 16 bytes (and rot_dim / 2 elements too), 16 bytes are moved at a time.
+ * rot_dim is even, 0 to min(head_dim, 256). */
+typedef struct KuHipRopeArgs {
+  uint32_t size; /* sizeof(KuHipRopeArgs) */
+  uint32_t dtype;
+  uint32_t layout;
+  uint32_t inverse;
+  float scale;
+  size_t tokens, q_heads, kv_heads, head_dim, rot_dim;
+  const double *freqs;      /* host memory, rot_dim / 2 */
+  const int32_t *positions; /* [tokens] */
+  const void *q;
+  int64_t q_token_stride, q_head_stride;
+  void *q_out;
+  int64_t q_out_token_stride, q_out_head_stride;
+  const void *k;
+  int64_t k_token_stride, k_head_stride;
+  void *k_out;
+  int64_t k_out_row_stride, k_out_head_stride;
+  const void *v;
+  int64_t v_token_stride, v_head_stride;
+  void *v_out;
+  int64_t v_out_row_stride, v_out_head_stride;
+  const int32_t *rows; /* [tokens] or NULL */
+  size_t out_rows;
+} KuHipRopeArgs;
+int32_t ku_hip_rope(const KuBackend *b, const KuHipRopeArgs *args, void *stream);
+
+/* ku_hip_sdpa_prefix: attention of a batch whose sequences share their first prefix_len keys.
+ *   out[b, t, h] = sum_j softmax_j(scale * q[b, t, h] . key_j) value_j
+ * over the prefix_len shared keys and values and those of sequence b's own own_lens[b] ones that query
+ * t sees: the q_len queries are the sequence's last q_len positions, so query t sees own key j when
+ * j < own_lens[b] - (q_len - 1 - t). q head h reads kv head h / (q_heads / kv_heads). The shared keys
+ * and values are read once for the whole batch. A query that sees no key gets zeros. Only keys that a
+ * query sees count: what other rows hold (infinities and NaN too) does not matter.
+ *   q, out  [batch, q_len, q_heads, head_dim], out not overlapping q
+ *   lse     [batch, q_len, q_heads] contiguous f32, or NULL: ln sum_j exp(scale * q . key_j), -inf for
+ *           a query that sees no key; outputs of several calls over parts of the keys join by it
+ *   prefix_k, prefix_v [prefix_len, kv_heads, head_dim] (prefix_len may be 0)
+ *   own_k, own_v [own_rows, kv_heads, head_dim]: own key j of sequence b is row b * own_seq_rows + j,
+ *           or with `pages` [batch, pages_per_seq] row pages[b][j / page_size] * page_size
+ *           + j % page_size (page_size a power of two; keys of a page whose index is outside
+ *           [0, own_rows / page_size) count as not there)
+ *   own_lens [batch], each taken into [0, own_max]; own_max (0: no own keys) sizes the launch
+ * k and v share their strides. head_dim is a multiple of 16 bytes, up to 128; pointers and strides
+ * are multiples of 16 bytes. scale is positive and finite.
+ *
+ * Partial results need ku_hip_sdpa_prefix_scratch(args) bytes (0: none; it depends on the sizes
+ * only). scratch NULL: a workspace of the backend that grows on demand, so such calls on one backend
+ * must be ordered on one stream, and a call under stream capture is refused if it needs any (the
+ * recorded graph would outlive the workspace). Calls, or graphs, that may overlap need a scratch each. */
+typedef struct KuHipSdpaPrefixArgs {
+  uint32_t size; /* sizeof(KuHipSdpaPrefixArgs) */
+  uint32_t dtype;
+  float scale;
+  size_t batch, q_len, q_heads, kv_heads, head_dim;
+  const void *q;
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  void *out;
+  int64_t out_batch_stride, out_token_stride, out_head_stride;
+  float *lse;
+  size_t prefix_len;
+  const void *prefix_k, *prefix_v;
+  int64_t prefix_row_stride, prefix_head_stride;
+  size_t own_max;
+  const int32_t *own_lens;
+  const void *own_k, *own_v;
+  int64_t own_row_stride, own_head_stride;
+  size_t own_rows, own_seq_rows;
+  const int32_t *pages;
+  size_t page_size, pages_per_seq;
+  void *scratch; /* 16-byte aligned */
+  size_t scratch_bytes;
+} KuHipSdpaPrefixArgs;
+int32_t ku_hip_sdpa_prefix(const KuBackend *b, const KuHipSdpaPrefixArgs *args, void *stream);
+/* Bytes of scratch ku_hip_sdpa_prefix needs for these arguments; SIZE_MAX (and ku_last_error) where it
+ * would refuse them. Needs no GPU. */
+size_t ku_hip_sdpa_prefix_scratch(const KuHipSdpaPrefixArgs *args);
+
+/* ku_hip_logits_adjust: penalties, biases and a grammar's mask on logits [rows, vocab], before
+ * softmax, sampling or argmax. For row r and token v, with n the times v was generated and s whether
+ * it occurs in the row's tokens at all:
+ *   y = x;  if (s) y = y > 0 ? y / repetition[r] : y * repetition[r];
+ *   y -= frequency[r] * n + (n > 0 ? presence[r] : 0);
+ *   y += the row's biases for v, in list order;   y = -inf unless the row's mask allows v
+ * in f32, rounded once to out_dtype.
+ *   tokens [rows, history] (row stride tokens_stride; 0 shares one list): the first lens[r] of a row
+ *          are its tokens, the first prompt_lens[r] of these its prompt, the others were generated.
+ *          lens NULL: history; prompt_lens NULL: 0; values are taken into range. Ids outside
+ *          [0, vocab) are ignored. tokens NULL: no history.
+ *   repetition (> 0), presence, frequency [rows] f32, each NULL for none
+ *   bias_ids i32, bias_values f32 [bias_count], bias_offsets i32 [rows + 1]: row r has entries
+ *          bias_offsets[r] to bias_offsets[r + 1] - 1 (taken into range). An id may repeat. NULL: none.
+ *   mask   [mask_rows, mask_stride words]: bit v % 32 of word v / 32 set = v is allowed. Row r goes by
+ *          mask row mask_index[r] (mask_index NULL: r); an index outside [0, mask_rows) leaves the row
+ *          unmasked. mask NULL: none.
+ * out may be logits itself (same dtype and stride), otherwise they may not overlap. */
+typedef struct KuHipLogitsArgs {
+  uint32_t size; /* sizeof(KuHipLogitsArgs) */
+  uint32_t dtype, out_dtype;
+  size_t rows, vocab;
+  const void *logits;
+  int64_t logits_stride;
+  void *out;
+  int64_t out_stride;
+  size_t history;
+  const int32_t *tokens;
+  int64_t tokens_stride;
+  const int32_t *lens, *prompt_lens;
+  const float *repetition, *presence, *frequency;
+  const int32_t *bias_ids;
+  const float *bias_values;
+  const int32_t *bias_offsets;
+  size_t bias_count;
+  const uint32_t *mask;
+  size_t mask_rows;
+  int64_t mask_stride;
+  const int32_t *mask_index;
+} KuHipLogitsArgs;
+int32_t ku_hip_logits_adjust(const KuBackend *b, const KuHipLogitsArgs *args, void *stream);
+
 /* Counters of a backend into out[0..cap): launches per kind (fused, gemm, attention, upload,
  * download), then plans built, constants uploaded and constants cached (plans and constants
  * are cached by graph content, so an equal graph rebuilt per call adds to neither); returns

@@ -15,7 +15,8 @@ from typing import Iterable, Sequence
 
 import numpy as np
 
-__all__ = ["DType", "Graph", "HipBackend", "Plan", "Tensor", "KuError", "lib", "amp", "amp_fp8", "KU_ERR"]
+__all__ = ["DType", "Graph", "HipBackend", "Plan", "Tensor", "KuError", "lib", "amp", "amp_fp8", "KU_ERR",
+           "RopeArgs", "SdpaPrefixArgs", "LogitsArgs", "rope_freqs", "sdpa_prefix_scratch"]
 
 _PKG = Path(__file__).resolve().parent
 _LIB_PATH = _PKG / "libkurumi_hip.so"
@@ -58,6 +59,100 @@ class DType(enum.IntEnum):
                          12: np.uint16, 13: np.float32, 14: np.float64, 15: np.complex64,
                          16: np.complex128}[int(self)])
 
+
+class _Args(C.Structure):
+    """A block of arguments of a call on device buffers: every field may be given by keyword, pointers
+    as ints (0 or None: null); `size` fills itself. Kept and reused between calls like the buffers."""
+
+    def __init__(self, **fields):
+        super().__init__()
+        self.size = C.sizeof(type(self))
+        for name, value in fields.items():
+            if not hasattr(type(self), name):
+                raise TypeError(f"{type(self).__name__} has no field {name!r}")
+            setattr(self, name, value)
+
+
+def _fields(text: str) -> list:
+    """ctypes fields from lines of "type: name name ..." in the struct's order."""
+    kinds = {"u32": C.c_uint32, "f32": C.c_float, "size": C.c_size_t, "stride": C.c_int64, "ptr": C.c_void_p,
+             "host_f64": C.POINTER(C.c_double)}
+    out = []
+    for line in text.strip().splitlines():
+        kind, names = line.split(":")
+        out += [(n, kinds[kind.strip()]) for n in names.split()]
+    return out
+
+
+class RopeArgs(_Args):
+    """KuHipRopeArgs (include/kurumi_hip.h): what `HipBackend.rope` takes."""
+    _fields_ = _fields("""
+        u32: size dtype layout inverse
+        f32: scale
+        size: tokens q_heads kv_heads head_dim rot_dim
+        host_f64: freqs
+        ptr: positions q
+        stride: q_token_stride q_head_stride
+        ptr: q_out
+        stride: q_out_token_stride q_out_head_stride
+        ptr: k
+        stride: k_token_stride k_head_stride
+        ptr: k_out
+        stride: k_out_row_stride k_out_head_stride
+        ptr: v
+        stride: v_token_stride v_head_stride
+        ptr: v_out
+        stride: v_out_row_stride v_out_head_stride
+        ptr: rows
+        size: out_rows""")
+
+
+class SdpaPrefixArgs(_Args):
+    """KuHipSdpaPrefixArgs (include/kurumi_hip.h): what `HipBackend.sdpa_prefix` takes."""
+    _fields_ = _fields("""
+        u32: size dtype
+        f32: scale
+        size: batch q_len q_heads kv_heads head_dim
+        ptr: q
+        stride: q_batch_stride q_token_stride q_head_stride
+        ptr: out
+        stride: out_batch_stride out_token_stride out_head_stride
+        ptr: lse
+        size: prefix_len
+        ptr: prefix_k prefix_v
+        stride: prefix_row_stride prefix_head_stride
+        size: own_max
+        ptr: own_lens own_k own_v
+        stride: own_row_stride own_head_stride
+        size: own_rows own_seq_rows
+        ptr: pages
+        size: page_size pages_per_seq
+        ptr: scratch
+        size: scratch_bytes""")
+
+
+class LogitsArgs(_Args):
+    """KuHipLogitsArgs (include/kurumi_hip.h): what `HipBackend.logits_adjust` takes."""
+    _fields_ = _fields("""
+        u32: size dtype out_dtype
+        size: rows vocab
+        ptr: logits
+        stride: logits_stride
+        ptr: out
+        stride: out_stride
+        size: history
+        ptr: tokens
+        stride: tokens_stride
+        ptr: lens prompt_lens repetition presence frequency bias_ids bias_values bias_offsets
+        size: bias_count
+        ptr: mask
+        size: mask_rows
+        stride: mask_stride
+        ptr: mask_index""")
+
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_UNSCALED, ROPE_LINEAR, ROPE_BASE, ROPE_BY_PARTS = 0, 1, 2, 3
 
 _lib = None
 
@@ -152,6 +247,12 @@ def _declare(L: C.CDLL) -> None:
         "ku_hip_profile": ([P, C.POINTER(C.c_uint64), sz], C.c_uint64),
         "ku_hip_linear_e4m3": ([P, P, u32, P, P, P, u32, sz, sz, sz, P], C.c_int32),
         "ku_hip_linear_e4m3_noalloc": ([P, u32, P, P, P, u32, sz, sz, sz, P], C.c_int32),
+        "ku_hip_rope_freqs": ([sz, C.c_double, u32, C.c_double, C.c_double, C.c_double, C.c_double,
+                               C.POINTER(C.c_double)], C.c_int32),
+        "ku_hip_rope": ([P, C.POINTER(RopeArgs), P], C.c_int32),
+        "ku_hip_sdpa_prefix": ([P, C.POINTER(SdpaPrefixArgs), P], C.c_int32),
+        "ku_hip_sdpa_prefix_scratch": ([C.POINTER(SdpaPrefixArgs)], sz),
+        "ku_hip_logits_adjust": ([P, C.POINTER(LogitsArgs), P], C.c_int32),
         "ku_quant_matmul": ([P, u32, u32, u32, u32, C.c_uint8, sz], u32),
         "ku_quantize": ([C.POINTER(C.c_float), sz, sz, C.c_uint8, sz, u32, C.c_char_p, C.POINTER(C.c_uint16),
                          C.POINTER(C.c_uint16)], None),
@@ -766,6 +867,21 @@ class HipBackend:
         """ku_hip_linear_e4m3_noalloc (static scratch, no allocation; m * k <= 16 MiB)."""
         linear_e4m3_noalloc(x, x_dtype, wq, sw, y, y_dtype, m, n, k, stream)
 
+    def rope(self, args: RopeArgs, stream: int | None = None) -> None:
+        """ku_hip_rope: rotary positions of q, k (and v copied) into q_out and the rows of a cache."""
+        if lib().ku_hip_rope(self.h, args, stream) != 0:
+            raise KuError(last_error())
+
+    def sdpa_prefix(self, args: SdpaPrefixArgs, stream: int | None = None) -> None:
+        """ku_hip_sdpa_prefix: attention over a shared prefix and each sequence's own keys."""
+        if lib().ku_hip_sdpa_prefix(self.h, args, stream) != 0:
+            raise KuError(last_error())
+
+    def logits_adjust(self, args: LogitsArgs, stream: int | None = None) -> None:
+        """ku_hip_logits_adjust: penalties for repeated tokens, biases and grammar masks on logits."""
+        if lib().ku_hip_logits_adjust(self.h, args, stream) != 0:
+            raise KuError(last_error())
+
     def compile(self, g: Graph, node: int) -> "Plan":
         """kurumi.h:456 ku_plan_compile on this backend (ku_hip_plan_compile_on)."""
         return Plan(g, node, self)
@@ -782,6 +898,23 @@ def linear_e4m3_noalloc(x: int, x_dtype: DType, wq: int, sw: int, y: int, y_dtyp
     """ku_hip_linear_e4m3_noalloc on device pointers (current device; no backend needed)."""
     if lib().ku_hip_linear_e4m3_noalloc(x, int(x_dtype), wq, sw, y, int(y_dtype), m, n, k, stream) != 0:
         raise KuError(f"ku_hip_linear_e4m3_noalloc: {last_error()}")
+
+
+def rope_freqs(rot_dim: int, base: float = 10000.0, scaling: int = ROPE_UNSCALED, factor: float = 1.0,
+               trained_len: float = 0.0, low: float = 1.0, high: float = 4.0):
+    """ku_hip_rope_freqs: the angular frequencies of rot_dim / 2 rotary pairs, as `RopeArgs.freqs` takes them."""
+    out = (C.c_double * max(rot_dim // 2, 1))()
+    if lib().ku_hip_rope_freqs(rot_dim, base, scaling, factor, trained_len, low, high, out) != 0:
+        raise KuError(last_error())
+    return out
+
+
+def sdpa_prefix_scratch(args: SdpaPrefixArgs) -> int:
+    """ku_hip_sdpa_prefix_scratch: bytes of scratch that `HipBackend.sdpa_prefix` needs for these arguments."""
+    n = lib().ku_hip_sdpa_prefix_scratch(args)
+    if n == C.c_size_t(-1).value:
+        raise KuError(last_error())
+    return n
 
 
 class Plan:

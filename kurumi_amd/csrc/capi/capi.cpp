@@ -12,6 +12,7 @@
 #include "../../../include/kurumi_hip.h"
 #include "../hip/backend.h"
 #include "../hip/kernels/kernels.h"
+#include "backend_handle.h"
 #include "errors.h"
 #include "handles.h"
 #include "../ir/graph.h"
@@ -25,7 +26,6 @@ using ku::Shape;
 // Plans keep the backend they were built on alive (shared ownership): a plan's steps use the
 // backend's stream, pools and constant cache, so freeing the KuBackend handle first only drops
 // the handle's reference and the backend ends with its last plan.
-struct KuBackend { std::shared_ptr<ku::hipbk::HipBackend> b; };
 struct KuPlan {
   std::shared_ptr<ku::hipbk::HipBackend> owner;  // null for the process-default backend
   std::shared_ptr<ku::hipbk::Plan> p;            // declared after owner: destroyed first
