@@ -2,22 +2,526 @@
 //
 //   out[b, t, h] = sum_j softmax_j(scale q[b, t, h] . K_j) V_j
 // over the shared prefix and the keys of sequence b that query t sees.
+//
+// The queries that read one kv head are the rows of a matrix product with its keys. Over the prefix
+// the rows of every sequence go through together ("pooled"): a key is read once for the whole batch,
+// which is what makes it a matrix product and not a vector one. A sequence's own keys meet its own rows
+// only. Where one sequence fills whole tiles of rows by itself (many queries), its tiles walk the prefix
+// and then its own keys in one pass ("joint").
+//
+// Tiles are computed transposed, so that one lane owns one query:
+//   S^T[key][q] = K[key][:] . Q[q][:],   O^T[d][q] += V^T[d][key] . P^T[key][q]
+// with 32 x 32 MFMA tiles. Lane l of an accumulator holds query l % 32 and rows 8 (v / 4) + 4 (l / 32)
+// + v % 4, so maximum, sum and rescale are a lane's own scalars, and the probabilities lie in registers
+// as the second product's operand. K and V go to LDS by DMA.
+//
+// The keys of a tile are cut into splits until the chip is full; each split leaves its maximum, sum and
+// unnormalised output in f32 in the scratch and a second kernel joins them in split order. A tile with
+// one split writes its output itself.
+//
+// Only rows that some query sees are ever loaded (places past the end repeat the last one), so what lies
+// behind them cannot matter. A query whose sums are not finite, or that saw nothing, is done again from
+// the definition by sdpa_one: an infinity or NaN in a value that another query of the tile sees, and a
+// page that is none, come out right that way.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "decode.h"
+#include "lds_dma.h"
 #include "sdpa_prefix.h"
 
 namespace ku::hipbk {
 
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((__vector_size__(4 * sizeof(short))));
+#define KU_LDS __attribute__((address_space(3)))
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// The running maximum moves only when a block exceeds it by more than this (in powers of two), so most
+// blocks leave O alone; probabilities reach 2^8 at most before they are normalised.
+constexpr float RESCALE = 8.f;
+
+// How a call is cut into work-groups.
+struct SdpaPlan {
+  bool joint = false;
+  // [0] the prefix with the rows of all sequences (joint: prefix and own keys of a sequence's rows);
+  // [1] a sequence's own keys with its rows
+  struct Part {
+    bool shared = false;  // four waves of 32 rows share the keys' blocks; else each wave is by itself
+    int tiles = 0, splits = 0;   // row tiles a kv head (and sequence), splits of their keys
+    int units = 0, groups = 0;   // tiles times splits of all of them, and work-groups: one unit each, or one a wave
+  } part[2];
+  int slots = 0;  // partial results a row
+};
+
+struct SdpaArgs {
+  SdpaDev a;
+  SdpaPlan p;
+  float* po;   // [rows][slots][D]
+  float2* ml;  // [rows][slots]: maximum in powers of two, sum
+};
+
 template <int DT>
-__global__ void __launch_bounds__(64) sdpa_rows_k(SdpaDev a) {
-  __shared__ float lds[kSdpaMaxDim];
-  const int64_t i = blockIdx.x;
-  sdpa_one<DT>(a, (int)(i / a.q_heads / a.q_len), (int)(i / a.q_heads % a.q_len), (int)(i % a.q_heads), lds);
+__device__ __forceinline__ void mfma_step(const u32x4& a, const u32x4& b, f32x16& c) {
+  if constexpr (DT == GT_BF16) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else if constexpr (DT == GT_F16) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const f32x2 v = {lo, hi};
+  if constexpr (DT == GT_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+template <int DT>
+__device__ __forceinline__ float sum2(uint32_t pair, float c) {
+  if constexpr (DT == GT_BF16) {
+    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), one, c, false);
+  } else {
+    const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), one, c, false);
+  }
+}
+// the value of the other half of the wave
+__device__ __forceinline__ float other_half(float x) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? sw[0] : sw[1]);
+}
+
+template <int DT, int D>
+struct Tile {
+  static constexpr int ES = DT == GT_F32 ? 4 : 2;
+  static constexpr int RB = D * ES;          // bytes of a row in LDS
+  static constexpr int CPR = RB / 16;        // 16-byte chunks of a row
+  static constexpr int KT = 32 * RB;         // bytes of 32 keys
+  static constexpr int DS = CPR / 2;         // chunk pairs: steps of S^T
+  static constexpr int DTL = D / 32;         // 32-row tiles of O^T
+  static constexpr int SB = DT == GT_F32 ? 1 : 2;  // 32-key tiles of a shared block
+  // shared: K and V, two buffers each; solo: K and V of every wave
+  static constexpr int LDS = std::max(4 * SB * KT, 4 * 2 * KT);
+  // rows r at one chunk: 16 of them on 16 bank groups of the 256-byte window
+  static __device__ __forceinline__ int kswz(int r) {
+    if constexpr (RB >= 256) return r & 15;
+    else return (r / (256 / RB)) % (16 / (256 / RB));
+  }
+  static __device__ __forceinline__ int vswz(int r) {
+    if constexpr (DT == GT_F32) return RB >= 256 ? ((r >> 2) & 1) * 8 : 0;
+    else if constexpr (RB >= 256) return 4 * (r & 3);
+    else return 4 * ((r / (256 / RB)) % (4 / (256 / RB)));
+  }
+};
+
+// One wave's 32 rows of a tile: Q fragments, running maximum, sum and O.
+template <int DT, int D>
+struct Rows {
+  using T = Tile<DT, D>;
+  u32x4 q[T::DS];
+  f32x16 o[T::DTL];
+  float m, l;  // m in powers of two, already times scale
+  int limit;   // own keys that this lane's query sees
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[t][v] = 0.f;
+  }
+  // `row`: this lane's query, or null past the last
+  __device__ __forceinline__ void load_q(const void* row, int dim) {
+    const int h = (threadIdx.x & 63) >> 5, chunks = dim * T::ES / 16;
+#pragma unroll
+    for (int s = 0; s < T::DS; ++s) {
+      const int c = 2 * s + h;
+      q[s] = u32x4{0, 0, 0, 0};
+      if (row && c < chunks) q[s] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(row) + c * 16);
+    }
+  }
+  // scores of 32 keys
+  __device__ __forceinline__ f32x16 scores(const KU_LDS unsigned char* K) const {
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    f32x16 s = {};
+#pragma unroll
+    for (int i = 0; i < T::DS; ++i) {
+      const u32x4 k = *(const KU_LDS u32x4*)(K + r * T::RB + (((2 * i + h) ^ T::kswz(r)) << 4));
+      mfma_step<DT>(k, q[i], s);
+    }
+    return s;
+  }
+  // keys from `left` on are not seen (left counts from the tile's first key)
+  static __device__ __forceinline__ void mask(f32x16& s, int left) {
+    const int lim = left - 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+      if ((v >> 2) * 8 + (v & 3) >= lim) s[v] = -INFINITY;
+  }
+  // the new maximum over NT tiles of scores, O and l brought to it
+  template <int NT>
+  __device__ __forceinline__ void rescale(const f32x16 (&s)[NT], float c) {
+    float bm = s[0][0];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) bm = fmaxf(bm, s[t][v]);
+    bm = fmaxf(bm, other_half(bm)) * c;
+    const bool need = bm > m + RESCALE || (bm > m && m == -INFINITY);
+    if (__builtin_amdgcn_ballot_w64(need) != 0) {
+      const float mn = need ? bm : m, corr = need ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+      m = mn;
+      l *= corr;
+#pragma unroll
+      for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[t][v] *= corr;
+    }
+  }
+  // O^T += V^T P^T over 32 keys; the sum adds the probabilities that the product uses
+  __device__ __forceinline__ void weigh(const f32x16& s, float c, const KU_LDS unsigned char* V) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const float em = m == -INFINITY ? 0.f : -m;  // nothing seen so far: every score is -inf
+    if constexpr (DT == GT_F32) {
+      const int r = lane & 31;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[v], c, em));
+        l += p;
+        const int key = (v >> 2) * 8 + (v & 3) + 4 * h;
+#pragma unroll
+        for (int t = 0; t < T::DTL; ++t) {
+          const int d = 32 * t + r;
+          const float x = *(const KU_LDS float*)(V + key * T::RB + (((d >> 2) ^ T::vswz(key)) << 4) + (d & 3) * 4);
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p, o[t], 0, 0, 0);
+        }
+      }
+    } else {
+      u32x4 p[2];
+      float rs[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * i], c, em));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], c, em));
+        const uint32_t pp = pack2<DT>(p0, p1);
+        rs[i & 1] = sum2<DT>(pp, rs[i & 1]);
+        p[i >> 2][i & 3] = pp;
+      }
+      l += rs[0] + rs[1];
+      // V^T fragments by transposing reads: in each 16-lane group input lane 4 k' + j points at key
+      // row k', dims 4 j.. + 3, and output lane i receives keys 0..3 of dim i; two of them fetch the
+      // keys that the probability registers hold, 16 s + 4 h + 0..3 and those + 8
+      const int g = lane >> 4, c16 = lane & 15;
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int t = 0; t < T::DTL; ++t) {
+          const int d = t * 32 + (g & 1) * 16 + (c16 & 3) * 4;
+          u32x2 half[2];
+#pragma unroll
+          for (int r2 = 0; r2 < 2; ++r2) {
+            const int kr = 16 * st + 8 * r2 + 4 * h + (c16 >> 2);
+            const KU_LDS unsigned char* a = V + kr * T::RB + (((d >> 3) ^ T::vswz(kr)) << 4) + (d & 7) * 2;
+            half[r2] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((KU_LDS s16x4*)a));
+          }
+          mfma_step<DT>(u32x4{half[0][0], half[0][1], half[1][0], half[1][1]}, p[st], o[t]);
+        }
+    }
+  }
+};
+
+// A run of keys of one kv head, prefix or own, and the DMA of tiles of it.
+template <int DT, int D>
+struct Keys {
+  using T = Tile<DT, D>;
+  const char *k, *v;   // row 0 of the head
+  int64_t stride;      // bytes a row
+  int n;               // keys that there are
+  const int32_t* table;  // pages, or null
+  int shift, npages;
+  bool none = false;   // a page that is none was met
+
+  // byte offset of key j's row
+  __device__ __forceinline__ int64_t offset(int j) {
+    j = j < n ? j : n - 1;
+    if (!table) return j * stride;
+    int32_t page = table[j >> shift];
+    if (page < 0 || page >= npages) {
+      none = true;
+      page = 0;
+    }
+    return (((int64_t)page << shift) + (j & ((1 << shift) - 1))) * stride;
+  }
+  // This wave's share (of `waves`) of the DMA of `keys` keys from key j0 into K and V tiles.
+  template <bool V, int KEYS, int WAVES>
+  __device__ __forceinline__ void load(int j0, KU_LDS unsigned char* dst, int wave, int dim) {
+    constexpr int N = KEYS * T::RB / 1024 / WAVES;
+    static_assert(N * WAVES * 1024 == KEYS * T::RB, "whole DMA pieces");
+    const int lane = threadIdx.x & 63, last = dim * T::ES / 16 - 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int blk = i * WAVES + wave, r = blk * (1024 / T::RB) + lane / T::CPR;
+      int c = (lane % T::CPR) ^ (V ? T::vswz(r) : T::kswz(r));
+      c = c < last ? c : last;  // features past head_dim meet zeros of Q, or are not stored
+      lds_dma16_g((V ? v : k) + offset(j0 + r) + c * 16, (KU_LDS void*)(dst + blk * 1024));
+    }
+  }
+};
+
+template <int DT, int D>
+__device__ __forceinline__ Keys<DT, D> prefix_keys(const SdpaDev& a, int kvh) {
+  using E = typename SdpaElem<DT>::T;
+  return {reinterpret_cast<const char*>(static_cast<const E*>(a.pk) + kvh * a.phead),
+          reinterpret_cast<const char*>(static_cast<const E*>(a.pv) + kvh * a.phead), a.prow * (int)sizeof(E), a.prefix, nullptr, 0, 0};
+}
+template <int DT, int D>
+__device__ __forceinline__ Keys<DT, D> own_keys(const SdpaDev& a, int b, int kvh) {
+  using E = typename SdpaElem<DT>::T;
+  const int64_t base = kvh * a.head + (a.page_shift < 0 ? b * a.seq_rows * a.row : 0);
+  return {reinterpret_cast<const char*>(static_cast<const E*>(a.k) + base), reinterpret_cast<const char*>(static_cast<const E*>(a.v) + base),
+          a.row * (int)sizeof(E), sdpa_len(a, b), a.page_shift < 0 ? nullptr : a.pages + b * a.per_seq,
+          a.page_shift < 0 ? 0 : a.page_shift, a.npages};
+}
+
+// Writes a wave's rows: `row` is this lane's (b, t, h) index or -1. With one slot a row the output
+// itself, else the partial result `slot`.
+template <int DT, int D>
+__device__ __forceinline__ void finish(const SdpaArgs& g, Rows<DT, D>& R, int64_t row, int slot, bool none, float* lds) {
+  using T = Tile<DT, D>;
+  const SdpaDev& a = g.a;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  float l = R.l + other_half(R.l);
+  if (none) l = NAN;
+  if (g.p.slots > 1) {
+    if (row < 0) return;
+    float* o = g.po + (row * g.p.slots + slot) * D;
+#pragma unroll
+    for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        *reinterpret_cast<f32x4*>(o + 32 * t + 8 * v + 4 * h) =
+            f32x4{R.o[t][4 * v], R.o[t][4 * v + 1], R.o[t][4 * v + 2], R.o[t][4 * v + 3]};
+    if (h == 0) g.ml[row * g.p.slots + slot] = make_float2(R.m, l);
+    return;
+  }
+  // 0 * x is not 0 for a sum that is not finite
+  float z = l * 0.f;
+#pragma unroll
+  for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) z = fmaf(R.o[t][v], 0.f, z);
+  z += other_half(z);
+  const bool bad = row >= 0 && (!(z == 0.f) || l == 0.f);
+  if (row >= 0 && !bad) {
+    const int64_t tok = row / a.q_heads;
+    const int b = (int)(tok / a.q_len), t0 = (int)(tok % a.q_len), head = (int)(row % a.q_heads);
+    using E = typename SdpaElem<DT>::T;
+    E* out = static_cast<E*>(a.o) + b * a.ob + t0 * a.ot + head * a.oh;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int d = 32 * t + 8 * v + 4 * h;
+        if (d >= a.dim) continue;
+        const float x[4] = {R.o[t][4 * v] * inv, R.o[t][4 * v + 1] * inv, R.o[t][4 * v + 2] * inv, R.o[t][4 * v + 3] * inv};
+        if constexpr (DT == GT_F32)
+          *reinterpret_cast<f32x4*>(out + d) = f32x4{x[0], x[1], x[2], x[3]};
+        else
+          *reinterpret_cast<u32x2*>(out + d) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+      }
+    if (a.lse && h == 0) a.lse[row] = (R.m + __builtin_amdgcn_logf(l)) * LN2;
+  }
+  uint32_t redo = (uint32_t)__builtin_amdgcn_ballot_w64(bad && h == 0);
+  while (redo) {
+    const int i = __builtin_ctz(redo);
+    redo &= redo - 1;
+    const int64_t r = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), i) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, i);
+    sdpa_one<DT>(a, (int)(r / a.q_heads / a.q_len), (int)(r / a.q_heads % a.q_len), (int)(r % a.q_heads), lds);
+  }
+}
+
+// blocks [first, last) of n that split i of s takes
+__device__ __forceinline__ void split_range(int n, int i, int s, int& first, int& last) {
+  first = (int)((int64_t)n * i / s);
+  last = (int)((int64_t)n * (i + 1) / s);
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) sdpa_tiles_k(SdpaArgs g) {
+  using T = Tile<DT, D>;
+  using E = typename SdpaElem<DT>::T;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[T::LDS];
+  KU_LDS unsigned char* lds = (KU_LDS unsigned char*)lds_raw;
+  const SdpaDev& a = g.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float c = a.scale * LOG2E;
+  int id = blockIdx.x;
+  const bool second = id >= g.p.part[0].groups;
+  const SdpaPlan::Part& part = g.p.part[second];
+  if (second) id -= g.p.part[0].groups;
+  const bool pooled = !g.p.joint && !second;
+
+  // the work-group's (sequence,) kv head, row tile and split
+  if (!part.shared) id = id * 4 + wave;
+  if (id >= part.units) return;  // all waves of a shared unit, or one by itself
+  const int tile = id % part.tiles;
+  id /= part.tiles;
+  const int split = id % part.splits;
+  id /= part.splits;
+  const int kvh = id % a.kv_heads, b = id / a.kv_heads;
+  const int per_seq = a.q_len * a.group, nrows = pooled ? a.batch * per_seq : per_seq;
+  const int r = tile * (part.shared ? 128 : 32) + (part.shared ? wave * 32 : 0) + (lane & 31);
+  Rows<DT, D> R;
+  int64_t row = -1;
+  const E* qrow = nullptr;
+  R.limit = 0;
+  if (r < nrows) {
+    const int seq = pooled ? r / per_seq : b, in = pooled ? r % per_seq : r, t = in / a.group, head = kvh * a.group + in % a.group;
+    row = ((int64_t)seq * a.q_len + t) * a.q_heads + head;
+    qrow = static_cast<const E*>(a.q) + seq * a.qb + t * a.qt + head * a.qh;
+    if (!pooled) R.limit = sdpa_len(a, b) - (a.q_len - 1 - t);
+  }
+  R.load_q(qrow, a.dim);
+  R.clear();
+
+  bool none = false;
+  // the tile's blocks: those of the prefix, then those of the sequence's own keys that its last row sees
+  const int bk = part.shared ? 32 * T::SB : 32;
+  const bool walks_own = second || g.p.joint;
+  int own_n = 0;
+  if (walks_own && a.own_max) {
+    const int last_row = std::min(tile * (part.shared ? 128 : 32) + (part.shared ? 127 : 31), nrows - 1);
+    own_n = std::max(0, sdpa_len(a, b) - (a.q_len - 1 - last_row / a.group));
+  }
+  const int np = second ? 0 : (a.prefix + bk - 1) / bk, no = (own_n + bk - 1) / bk;
+  int first, last;
+  split_range(np + no, split, part.splits, first, last);
+  Keys<DT, D> P = prefix_keys<DT, D>(a, kvh), O = own_keys<DT, D>(a, walks_own ? b : 0, kvh);
+  if (!a.own_max) O.n = 0;
+
+  if (part.shared) {
+    constexpr int BK = 32 * T::SB, TB = T::SB * T::KT;
+    auto kbuf = [&](int i) { return lds + i * TB; };
+    auto vbuf = [&](int i) { return lds + (2 + i) * TB; };
+    auto fetch = [&](int blk) {
+      Keys<DT, D>& S = blk < np ? P : O;
+      const int j0 = (blk < np ? blk : blk - np) * BK;
+      S.template load<false, BK, 4>(j0, kbuf(blk & 1), wave, a.dim);
+      S.template load<true, BK, 4>(j0, vbuf(blk & 1), wave, a.dim);
+    };
+    if (first < last) fetch(first);
+    for (int blk = first; blk < last; ++blk) {
+      vm_wait<0>();
+      __syncthreads();
+      if (blk + 1 < last) fetch(blk + 1);
+      const bool pre = blk < np;
+      const int j0 = (pre ? blk : blk - np) * BK;
+      f32x16 s[T::SB];
+#pragma unroll
+      for (int t = 0; t < T::SB; ++t) s[t] = R.scores(kbuf(blk & 1) + t * T::KT);
+      const int lim = pre ? a.prefix : R.limit;
+      if (!pre || j0 + BK > a.prefix)
+#pragma unroll
+        for (int t = 0; t < T::SB; ++t) R.mask(s[t], lim - j0 - 32 * t);
+      R.rescale(s, c);
+#pragma unroll
+      for (int t = 0; t < T::SB; ++t) R.weigh(s[t], c, vbuf(blk & 1) + t * T::KT);
+    }
+    __syncthreads();
+  } else {
+    KU_LDS unsigned char *K = lds + wave * 2 * T::KT, *V = K + T::KT;
+    for (int blk = first; blk < last; ++blk) {
+      const bool pre = blk < np;
+      const int j0 = (pre ? blk : blk - np) * 32;
+      Keys<DT, D>& S = pre ? P : O;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      S.template load<false, 32, 1>(j0, K, 0, a.dim);
+      S.template load<true, 32, 1>(j0, V, 0, a.dim);
+      vm_wait<0>();
+      asm volatile("" ::: "memory");
+      f32x16 s[1];
+      s[0] = R.scores(K);
+      const int lim = pre ? a.prefix : R.limit;
+      if (!pre || j0 + 32 > a.prefix) R.mask(s[0], lim - j0);
+      R.rescale(s, c);
+      R.weigh(s[0], c, V);
+    }
+  }
+  none = __builtin_amdgcn_ballot_w64(O.none) != 0;
+  if (part.shared && O.table) {  // any wave of the group may have met it
+    int* flag = reinterpret_cast<int*>(lds_raw);
+    if (threadIdx.x == 0) *flag = 0;
+    __syncthreads();
+    if (none && lane == 0) atomicOr(flag, 1);
+    __syncthreads();
+    none = *flag != 0;
+    __syncthreads();
+  }
+  finish<DT, D>(g, R, row, second ? g.p.part[0].splits + split : split, none,
+                reinterpret_cast<float*>(lds_raw + wave * 2 * T::KT));
+}
+
+// Joins the partial results of a row, one wave a row.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
+  __shared__ float lds[4][kSdpaMaxDim];
+  const SdpaDev& a = g.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= (int64_t)a.batch * a.q_len * a.q_heads) return;
+  const float2* ml = g.ml + row * g.p.slots;
+  const int n = g.p.slots;
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[i].x);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  constexpr int C = D / 32 < 2 ? 1 : D / 64;  // values a lane
+  float l = 0.f, acc[C] = {};
+  for (int i = 0; i < n; ++i) {
+    const float2 x = ml[i];
+    if (x.x == -INFINITY && x.y == 0.f) continue;  // saw nothing: its output was not summed
+    const float w = __builtin_amdgcn_exp2f(x.x - m);
+    l = fmaf(w, x.y, l);
+    const float* o = g.po + (row * n + i) * D + lane * C;
+    if (D >= 64 || lane < 32)
+#pragma unroll
+      for (int k = 0; k < C; ++k) acc[k] = fmaf(w, o[k], acc[k]);
+  }
+  float z = l * 0.f;
+#pragma unroll
+  for (int k = 0; k < C; ++k) z = fmaf(acc[k], 0.f, z);
+  const int64_t tok = row / a.q_heads;
+  const int b = (int)(tok / a.q_len), t = (int)(tok % a.q_len), head = (int)(row % a.q_heads);
+  if (__builtin_amdgcn_ballot_w64(!(z == 0.f)) != 0 || l == 0.f) {
+    sdpa_one<DT>(a, b, t, head, lds[wave]);
+    return;
+  }
+  using E = typename SdpaElem<DT>::T;
+  E* out = static_cast<E*>(a.o) + b * a.ob + t * a.ot + head * a.oh;
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+    if (lane * C + k < a.dim) out[lane * C + k] = store_elem<DT, E>(acc[k] * inv);
+  if (a.lse && lane == 0) a.lse[row] = (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 SdpaDev device_args(const KuHipSdpaPrefixArgs& a) {
@@ -55,6 +559,53 @@ SdpaDev device_args(const KuHipSdpaPrefixArgs& a) {
   d.npages = a.pages ? (int32_t)(a.own_rows / a.page_size) : 0;
   d.scale = a.scale;
   return d;
+}
+
+// Whether one sequence's rows fill tiles of 128 well enough to walk the prefix by themselves; where they
+// do not, the sequences' rows share tiles over the prefix.
+SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
+  SdpaPlan p;
+  const int64_t per_seq = (int64_t)(a.q_len * (a.q_heads / a.kv_heads)), kv = (int64_t)a.kv_heads, nb = (int64_t)a.batch;
+  const bool f32 = a.dtype == KU_F32;
+  const int64_t bk_shared = f32 ? 32 : 64;
+  const int64_t full = (per_seq + 127) / 128 * 128;
+  p.joint = full * 4 <= per_seq * 5;
+  auto cut = [&](SdpaPlan::Part& part, int64_t rows, int64_t items, int64_t keys) {
+    if (keys == 0 || items == 0 || rows == 0) return;
+    part.shared = rows > 32;
+    part.tiles = (int)((rows + (part.shared ? 127 : 31)) / (part.shared ? 128 : 32));
+    const int64_t blocks = (keys + (part.shared ? bk_shared : 32) - 1) / (part.shared ? bk_shared : 32);
+    const int64_t want = (part.shared ? 2 : 8) * (int64_t)cu_count();  // work-groups, or waves
+    part.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / (items * part.tiles), (blocks + 1) / 2, 256}));
+    part.units = (int)(items * part.tiles * part.splits);
+    part.groups = part.shared ? part.units : (part.units + 3) / 4;
+  };
+  if (p.joint) {
+    cut(p.part[0], per_seq, nb * kv, (int64_t)(a.prefix_len + a.own_max));
+  } else {
+    cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len);
+    cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max);
+  }
+  p.slots = p.part[0].splits + p.part[1].splits;
+  return p;
+}
+
+int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+template <int DT, int D>
+void launch_d(const SdpaArgs& g, hipStream_t s) {
+  const unsigned groups = (unsigned)(g.p.part[0].groups + g.p.part[1].groups);
+  if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D>), dim3(groups), dim3(256), 0, s, g);
+  const int64_t rows = (int64_t)g.a.batch * g.a.q_len * g.a.q_heads;
+  if (g.p.slots != 1) hipLaunchKernelGGL((sdpa_join_k<DT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, g);
+}
+template <int DT>
+void launch_t(const SdpaArgs& g, int d, hipStream_t s) {
+  switch (d) {
+    case 32: launch_d<DT, 32>(g, s); break;
+    case 64: launch_d<DT, 64>(g, s); break;
+    default: launch_d<DT, 128>(g, s); break;
+  }
 }
 
 }  // namespace
@@ -119,16 +670,24 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
   }
 }
 
-size_t sdpa_prefix_scratch_bytes(const KuHipSdpaPrefixArgs&) { return 0; }
+size_t sdpa_prefix_scratch_bytes(const KuHipSdpaPrefixArgs& a) {
+  const SdpaPlan p = make_plan(a);
+  if (a.batch == 0 || p.slots <= 1) return 0;
+  return a.batch * a.q_len * a.q_heads * (size_t)p.slots * (padded_dim(a.head_dim) * sizeof(float) + sizeof(float2));
+}
 
-void launch_sdpa_prefix(const KuHipSdpaPrefixArgs& a, void*, hipStream_t s) {
+void launch_sdpa_prefix(const KuHipSdpaPrefixArgs& a, void* scratch, hipStream_t s) {
   if (a.batch == 0) return;
-  const SdpaDev d = device_args(a);
-  const dim3 grid((unsigned)(a.batch * a.q_len * a.q_heads));
+  SdpaArgs g;
+  g.a = device_args(a);
+  g.p = make_plan(a);
+  const int d = padded_dim(a.head_dim);
+  g.po = static_cast<float*>(scratch);
+  g.ml = reinterpret_cast<float2*>(g.po + a.batch * a.q_len * a.q_heads * (size_t)g.p.slots * d);
   switch (a.dtype) {
-    case KU_BF16: hipLaunchKernelGGL((sdpa_rows_k<GT_BF16>), grid, dim3(64), 0, s, d); break;
-    case KU_F16: hipLaunchKernelGGL((sdpa_rows_k<GT_F16>), grid, dim3(64), 0, s, d); break;
-    default: hipLaunchKernelGGL((sdpa_rows_k<GT_F32>), grid, dim3(64), 0, s, d); break;
+    case KU_BF16: launch_t<GT_BF16>(g, d, s); break;
+    case KU_F16: launch_t<GT_F16>(g, d, s); break;
+    default: launch_t<GT_F32>(g, d, s); break;
   }
   check_launch();
 }
