@@ -9,6 +9,7 @@
 // fraction is then exact enough in f32 for sine and cosine to half a step of f32.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "decode.h"
@@ -32,53 +33,136 @@ struct RopeDev {
   const int32_t* positions;
   const int32_t* rows;
   int64_t tokens, out_rows;
-  int q_heads, kv_heads, head_dim, rot;
+  uint32_t dim, rot;
+  uint32_t turned, copied, v_units;    // units of a q or k head: turned ones, then copied ones; of a v head
+  uint32_t q_units, qk_units, units;   // units a token: up to the last q head, k head, v head
+  uint32_t block_tokens, block_units;  // what a work-group takes
   float scale;
   double turns[kMaxPairs];  // f_i / 2 pi, negated for the inverse
 };
 
-template <int DT, class T>
-__device__ __forceinline__ float ld(const T* p) { return load_elem<DT, T, float>(*p); }
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;  // units a thread has in flight
 
-// One work-group per (token, head): heads are q's, then k's, then v's.
-template <int DT, class T, bool HALF>
-__global__ void __launch_bounds__(64) rope_k(RopeDev a) {
-  const int64_t t = blockIdx.x;
-  int h = blockIdx.y;
-  const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
-  const RopeSide& sd = is_q ? a.q : is_v ? a.v : a.k;
-  h = is_q ? h : is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
-  if (!sd.in) return;
-  int64_t row = t;
-  if (!is_q) {
-    if (a.rows) row = a.rows[t];
-    if (row < 0 || row >= a.out_rows) return;
+template <int N>
+struct Bits;
+template <> struct Bits<2> { using T = uint16_t; };
+template <> struct Bits<4> { using T = uint32_t; };
+template <> struct Bits<16> { using T = uint4; };
+
+// A unit is two vectors of V elements of one head: the low and the high features of V pairs (half
+// layout: i and i + rot / 2; interleaved: next to each other), or up to two vectors that are copied.
+// A work-group takes block_tokens tokens; it forms their angles once, in LDS, for all heads: a sine and
+// cosine of a 64-bit angle for each unit of each head would take longer than moving the unit.
+// 8192 tokens of 48 heads of 128, bf16: see the table of the kernel's cases.
+template <int DT, class T, int V, bool HALF>
+__global__ void __launch_bounds__(kThreads) rope_k(RopeDev a) {
+  using W = typename Bits<V * (int)sizeof(T)>::T;
+  extern __shared__ float2 table[];  // [block_tokens][rot / 2]: cosine, sine, times scale
+  const int64_t t0 = (int64_t)blockIdx.x * a.block_tokens;
+  const uint32_t nt = (uint32_t)(a.tokens - t0 < a.block_tokens ? a.tokens - t0 : a.block_tokens);
+  const uint32_t first = blockIdx.y * a.block_units;
+  const uint32_t per_token = a.units - first < a.block_units ? a.units - first : a.block_units;
+  const uint32_t total = nt * per_token, half = a.rot / 2;
+
+  struct Unit {
+    W x[2];
+    T* y;           // null: nothing to store
+    uint32_t hi;    // element offset of the second vector; 0: there is none
+    uint32_t pair;  // table entry of the first pair, or ~0 for a copy
+  };
+  auto load = [&](uint32_t u) {
+    Unit r{};
+    const uint32_t t = u / per_token;
+    uint32_t i = u - t * per_token + first, head, unit, lo;
+    const bool is_q = i < a.q_units, is_v = i >= a.qk_units;
+    const RopeSide& sd = is_q ? a.q : is_v ? a.v : a.k;
+    i -= is_q ? 0 : is_v ? a.qk_units : a.q_units;
+    const uint32_t each = is_v ? a.v_units : a.turned + a.copied;
+    head = i / each;
+    unit = i - head * each;
+    int64_t row = t0 + t;
+    if (!is_q && a.rows) row = a.rows[t0 + t];
+    if (!is_q && (row < 0 || row >= a.out_rows)) return r;
+    if (!is_v && unit < a.turned) {
+      r.pair = t * half + unit * V;
+      lo = HALF ? unit * V : 2 * unit * V;
+      r.hi = HALF ? half : V;
+    } else {
+      r.pair = ~0u;
+      lo = is_v ? 2 * unit * V : a.rot + 2 * (unit - a.turned) * V;
+      if (lo >= a.dim) return r;  // a head of an odd number of copied vectors next to turned ones
+      r.hi = lo + V < a.dim ? V : 0;
+    }
+    const T* x = static_cast<const T*>(sd.in) + (t0 + t) * sd.in_token + head * sd.in_head + lo;
+    r.y = static_cast<T*>(sd.out) + row * sd.out_row + head * sd.out_head + lo;
+    r.x[0] = *reinterpret_cast<const W*>(x);
+    if (r.hi) r.x[1] = *reinterpret_cast<const W*>(x + r.hi);
+    return r;
+  };
+  auto store = [&](Unit& r) {
+    if (!r.y) return;
+    if (r.pair != ~0u) {
+      T e[2][V];
+      __builtin_memcpy(e, r.x, sizeof(e));
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float2 cs = table[r.pair + i];
+        // half layout: pair i of the unit is (e[0][i], e[1][i]); interleaved: elements 2 i, 2 i + 1 of both
+        T& lo = HALF ? e[0][i] : e[(2 * i) / V][(2 * i) % V];
+        T& hi = HALF ? e[1][i] : e[(2 * i + 1) / V][(2 * i + 1) % V];
+        const float xl = load_elem<DT, T, float>(lo), xh = load_elem<DT, T, float>(hi);
+        lo = store_elem<DT, T>(fmaf(xl, cs.x, -xh * cs.y));
+        hi = store_elem<DT, T>(fmaf(xh, cs.x, xl * cs.y));
+      }
+      __builtin_memcpy(r.x, e, sizeof(e));
+    }
+    *reinterpret_cast<W*>(r.y) = r.x[0];
+    if (r.hi) *reinterpret_cast<W*>(r.y + r.hi) = r.x[1];
+  };
+
+  Unit unit[kUnroll];
+  for (uint32_t base = threadIdx.x; base < total + threadIdx.x; base += kThreads * kUnroll) {
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      unit[j].y = nullptr;
+      if (base + kThreads * j < total) unit[j] = load(base + kThreads * j);
+    }
+    if (base == threadIdx.x) {  // the first loads are on their way
+      for (uint32_t i = threadIdx.x; i < nt * half; i += kThreads) {
+        const uint32_t t = i / half;
+        const double turns = (double)a.positions[t0 + t] * a.turns[i - t * half];
+        float sn, cs;
+        sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+        table[i] = make_float2(cs * a.scale, sn * a.scale);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) store(unit[j]);
   }
-  const T* x = static_cast<const T*>(sd.in) + t * sd.in_token + h * sd.in_head;
-  T* y = static_cast<T*>(sd.out) + row * sd.out_row + h * sd.out_head;
-  const int rot = is_v ? 0 : a.rot;
-  const double p = rot ? (double)a.positions[t] : 0.0;
-  for (int i = threadIdx.x; i < rot / 2; i += 64) {
-    const double turns = p * a.turns[i];
-    float sn, cs;
-    sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
-    sn *= a.scale;
-    cs *= a.scale;
-    const int lo = HALF ? i : 2 * i, hi = HALF ? i + rot / 2 : 2 * i + 1;
-    const float xl = ld<DT>(x + lo), xh = ld<DT>(x + hi);
-    y[lo] = store_elem<DT, T>(fmaf(xl, cs, -xh * sn));
-    y[hi] = store_elem<DT, T>(fmaf(xh, cs, xl * sn));
-  }
-  for (int i = rot + threadIdx.x; i < a.head_dim; i += 64) y[i] = x[i];
 }
 
-template <int DT, class T>
-void launch_t(const RopeDev& d, bool half, hipStream_t s) {
-  const dim3 grid((unsigned)d.tokens, (unsigned)(d.q_heads + 2 * d.kv_heads));
+template <int DT, class T, int V>
+void launch_v(RopeDev& d, uint32_t q_heads, uint32_t k_heads, uint32_t v_heads, bool half, hipStream_t s) {
+  auto units = [](uint32_t features) { return (features + 2 * V - 1) / (2 * V); };
+  d.turned = d.rot / 2 / V;
+  d.copied = units(d.dim - d.rot);
+  d.v_units = units(d.dim);
+  d.q_units = q_heads * (d.turned + d.copied);
+  d.qk_units = d.q_units + k_heads * (d.turned + d.copied);
+  d.units = d.qk_units + v_heads * d.v_units;
+  // Work-groups of about 8 units a thread (two rounds of loads) where that leaves enough of them, of
+  // one where it does not: a few tokens are spread over their heads.
+  const int64_t all = d.tokens * (int64_t)d.units, want = all / (8 * kThreads) >= 4 * (int64_t)cu_count() ? 8 * kThreads : kThreads;
+  d.block_tokens = (uint32_t)std::max<int64_t>(1, std::min<int64_t>({want / d.units, d.tokens, 64}));
+  d.block_units = d.block_tokens > 1 ? d.units : (uint32_t)std::min<int64_t>(d.units, std::max<int64_t>(want, (d.units + 65534) / 65535));
+  const dim3 grid((unsigned)((d.tokens + d.block_tokens - 1) / d.block_tokens), (d.units + d.block_units - 1) / d.block_units);
+  const size_t lds = d.block_tokens * (d.rot / 2) * sizeof(float2);
   if (half)
-    hipLaunchKernelGGL((rope_k<DT, T, true>), grid, dim3(64), 0, s, d);
+    hipLaunchKernelGGL((rope_k<DT, T, V, true>), grid, dim3(kThreads), lds, s, d);
   else
-    hipLaunchKernelGGL((rope_k<DT, T, false>), grid, dim3(64), 0, s, d);
+    hipLaunchKernelGGL((rope_k<DT, T, V, false>), grid, dim3(kThreads), lds, s, d);
 }
 
 }  // namespace
@@ -161,17 +245,31 @@ void launch_rope(const KuHipRopeArgs& a, hipStream_t s) {
   d.rows = a.rows;
   d.tokens = (int64_t)a.tokens;
   d.out_rows = (int64_t)a.out_rows;
-  d.q_heads = a.q ? (int)a.q_heads : 0;
-  d.kv_heads = a.k || a.v ? (int)a.kv_heads : 0;
-  d.head_dim = (int)a.head_dim;
-  d.rot = a.q || a.k ? (int)a.rot_dim : 0;
+  d.dim = (uint32_t)a.head_dim;
+  d.rot = a.q || a.k ? (uint32_t)a.rot_dim : 0;
   d.scale = a.scale;
-  for (int i = 0; i < d.rot / 2; ++i) d.turns[i] = (a.inverse ? -a.freqs[i] : a.freqs[i]) / 6.283185307179586476925;
+  for (uint32_t i = 0; i < d.rot / 2; ++i) d.turns[i] = (a.inverse ? -a.freqs[i] : a.freqs[i]) / 6.283185307179586476925;
+  const uint32_t qh = a.q ? (uint32_t)a.q_heads : 0, kh = a.k ? (uint32_t)a.kv_heads : 0, vh = a.v ? (uint32_t)a.kv_heads : 0;
   const bool half = a.layout == KU_ROPE_HALF;
+  // 16 bytes at a time where everything is made of them
+  const int64_t v = a.dtype == KU_F32 ? 4 : 8;
+  bool wide = d.dim % v == 0 && (d.rot / 2) % v == 0;
+  for (const RopeSide* x : {&d.q, &d.k, &d.v})
+    if (x->in)
+      wide = wide && aligned_to(x->in, 16) && aligned_to(x->out, 16) && x->in_token % v == 0 && x->in_head % v == 0 &&
+             x->out_row % v == 0 && x->out_head % v == 0;
+  auto go = [&](auto dt, auto elem) {
+    constexpr int DT = decltype(dt)::value;
+    using T = decltype(elem);
+    if (wide)
+      launch_v<DT, T, 16 / (int)sizeof(T)>(d, qh, kh, vh, half, s);
+    else
+      launch_v<DT, T, 1>(d, qh, kh, vh, half, s);
+  };
   switch (a.dtype) {
-    case KU_BF16: launch_t<GT_BF16, uint16_t>(d, half, s); break;
-    case KU_F16: launch_t<GT_F16, uint16_t>(d, half, s); break;
-    default: launch_t<GT_F32, float>(d, half, s); break;
+    case KU_BF16: go(DTag<GT_BF16>{}, uint16_t{}); break;
+    case KU_F16: go(DTag<GT_F16>{}, uint16_t{}); break;
+    default: go(DTag<GT_F32>{}, float{}); break;
   }
   check_launch();
 }
