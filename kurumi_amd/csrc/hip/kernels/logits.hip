@@ -5,8 +5,9 @@
 // with n the times a token was generated in the row and seen whether it occurs in its tokens at all.
 //
 // A work-group takes a chunk of one row's vocabulary and counts, in LDS, the row's tokens that fall
-// into it: whole numbers, so the order of the atomics does not matter. Bit 31 of a counter says that
-// the token is in the prompt, the others count how often it was generated.
+// into it: whole numbers, so the order of the atomics does not matter. Nothing the size of the
+// vocabulary is kept or cleared in memory; every logit is read once and written once, and the row's
+// tokens and biases are read again (from L2) by each of its chunks.
 #include <hip/hip_runtime.h>
 
 #include "decode.h"
@@ -17,8 +18,10 @@ namespace ku::hipbk {
 
 namespace {
 
-constexpr int kThreads = 256, kChunk = 4096;
-constexpr uint32_t kInPrompt = 0x80000000u;
+constexpr int kThreads = 512, kVec = 8, kPerThread = 2;  // a thread's logits: two vectors of 8
+constexpr int kChunk = kThreads * kVec * kPerThread;
+// A counter: how often the token was generated, and whether it is in the prompt and has biases.
+constexpr uint32_t kInPrompt = 0x80000000u, kBiased = 0x40000000u, kCount = kBiased - 1;
 
 struct LogitsDev {
   const void* x;
@@ -37,59 +40,116 @@ struct LogitsDev {
 
 __device__ __forceinline__ int32_t clamped(int32_t v, int32_t hi) { return v < 0 ? 0 : v > hi ? hi : v; }
 
+// kVec logits from (to) element alignment: rows of an odd vocabulary start anywhere.
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+  T e[kVec];
+};
+
 template <int DT, class T, int OT, class O>
 __global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
-  __shared__ uint32_t count[kChunk];
-  __shared__ float val[kChunk];
+  __shared__ __attribute__((aligned(16))) uint32_t count[kChunk];
+  __shared__ float bias[kChunk];
+  __shared__ int repeats;
   const int64_t r = blockIdx.x / a.chunks, c0 = (int64_t)(blockIdx.x % a.chunks) * kChunk;
   const int n = (int)(a.vocab - c0 < kChunk ? a.vocab - c0 : kChunk), tid = threadIdx.x;
-  for (int i = tid; i < n; i += kThreads) count[i] = 0;
-  __syncthreads();
-  if (a.tokens) {
-    const int32_t len = a.lens ? clamped(a.lens[r], a.history) : a.history;
-    const int32_t prompt = a.prompt_lens ? clamped(a.prompt_lens[r], len) : 0;
-    const int32_t* tok = a.tokens + r * a.ts;
-    for (int32_t i = tid; i < len; i += kThreads) {
-      const int64_t at = (int64_t)tok[i] - c0;
-      if (at < 0 || at >= n) continue;
-      if (i < prompt)
-        atomicOr(&count[at], kInPrompt);
-      else
-        atomicAdd(&count[at], 1u);
+  const T* x = static_cast<const T*>(a.x) + r * a.xs + c0;
+  O* y = static_cast<O*>(a.y) + r * a.ys + c0;
+
+  // the logits are on their way while the tokens are counted
+  Vec<T> in[kPerThread];
+#pragma unroll
+  for (int j = 0; j < kPerThread; ++j) {
+    const int i = (j * kThreads + tid) * kVec;
+    if (i + kVec <= n) {
+      in[j] = *reinterpret_cast<const Vec<T>*>(x + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (i + e < n) in[j].e[e] = x[i + e];
     }
   }
-  __syncthreads();
-  const float rep = a.repetition ? a.repetition[r] : 1.f, pres = a.presence ? a.presence[r] : 0.f,
-              freq = a.frequency ? a.frequency[r] : 0.f;
-  const T* x = static_cast<const T*>(a.x) + r * a.xs + c0;
-  for (int i = tid; i < n; i += kThreads) {
-    float v = load_elem<DT, T, float>(x[i]);
-    const uint32_t c = count[i];
-    if (c) {
-      v = v > 0.f ? v / rep : v * rep;
-      const uint32_t g = c & ~kInPrompt;
-      if (g) v -= fmaf(freq, (float)g, pres);
-    }
-    val[i] = v;
+  int32_t len = 0, prompt = 0, e0 = 0, e1 = 0;
+  if (a.tokens) {
+    len = a.lens ? clamped(a.lens[r], a.history) : a.history;
+    prompt = a.prompt_lens ? clamped(a.prompt_lens[r], len) : 0;
   }
   if (a.bias_ids) {
-    // an id's entries all go to the thread that holds its logit, in list order
-    const int32_t e0 = clamped(a.bias_offsets[r], a.bias_count), e1 = clamped(a.bias_offsets[r + 1], a.bias_count);
-    for (int32_t e = e0; e < e1; ++e) {
-      const int64_t at = (int64_t)a.bias_ids[e] - c0;
-      if (at >= 0 && at < n && at % kThreads == tid) val[at] += a.bias_values[e];
-    }
+    e0 = clamped(a.bias_offsets[r], a.bias_count);
+    e1 = clamped(a.bias_offsets[r + 1], a.bias_count);
   }
-  const uint32_t* bits = nullptr;
+  const float rep = a.repetition ? a.repetition[r] : 1.f, pres = a.presence ? a.presence[r] : 0.f,
+              freq = a.frequency ? a.frequency[r] : 0.f;
+  const uint8_t* bits = nullptr;
   if (a.mask) {
     const int64_t m = a.mask_index ? a.mask_index[r] : r;
-    if (m >= 0 && m < a.mask_rows) bits = a.mask + m * a.ms + c0 / 32;
+    if (m >= 0 && m < a.mask_rows) bits = reinterpret_cast<const uint8_t*>(a.mask + m * a.ms) + c0 / 8;
   }
-  O* y = static_cast<O*>(a.y) + r * a.ys + c0;
-  for (int i = tid; i < n; i += kThreads) {
-    float v = val[i];
-    if (bits && !(bits[i >> 5] >> (i & 31) & 1)) v = -INFINITY;
-    y[i] = store_elem<OT, O>(v);
+  const bool counts = len > 0 || e1 > e0;
+  if (counts) {
+#pragma unroll
+    for (int i = 0; i < kChunk / 4 / kThreads; ++i) reinterpret_cast<uint4*>(count)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) repeats = 0;
+    __syncthreads();
+    const int32_t* tok = a.tokens + r * a.ts;
+    for (int32_t i0 = 0; i0 < len; i0 += 4 * kThreads) {
+      int32_t id[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) id[j] = i0 + j * kThreads + tid < len ? tok[i0 + j * kThreads + tid] : -1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = (int64_t)id[j] - c0;
+        if (at < 0 || at >= n) continue;
+        if (i0 + j * kThreads + tid < prompt)
+          atomicOr(&count[at], kInPrompt);
+        else
+          atomicAdd(&count[at], 1u);
+      }
+    }
+    // an id of a row's biases comes once as a rule: its bias is put down by the thread that reads it
+    for (int32_t e = e0 + tid; e < e1; e += kThreads) {
+      const int64_t at = (int64_t)a.bias_ids[e] - c0;
+      if (at < 0 || at >= n) continue;
+      if (atomicOr(&count[at], kBiased) & kBiased) repeats = 1;
+      bias[at] = a.bias_values[e];
+    }
+    __syncthreads();
+    if (repeats) {
+      // some come again: each thread sums those of its places (at % kThreads) in list order
+      for (int i = tid; i < n; i += kThreads) bias[i] = 0.f;
+      for (int32_t e = e0; e < e1; ++e) {
+        const int64_t at = (int64_t)a.bias_ids[e] - c0;
+        if (at >= 0 && at < n && at % kThreads == tid) bias[at] += a.bias_values[e];
+      }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kPerThread; ++j) {
+    const int i = (j * kThreads + tid) * kVec;
+    if (i >= n) break;
+    const uint32_t allowed = bits ? bits[i / 8] : 0xffu;
+    Vec<O> out;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      float v = load_elem<DT, T, float>(in[j].e[e]);
+      const uint32_t c = counts ? count[i + e] : 0;
+      if (c) {
+        const uint32_t g = c & kCount;
+        if (c & ~kBiased) v = v > 0.f ? v / rep : v * rep;
+        if (g) v -= fmaf(freq, (float)g, pres);
+        if (c & kBiased) v += bias[i + e];
+      }
+      if (!(allowed >> e & 1)) v = -INFINITY;
+      out.e[e] = store_elem<OT, O>(v);
+    }
+    if (i + kVec <= n) {
+      *reinterpret_cast<Vec<O>*>(y + i) = out;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (i + e < n) y[i + e] = out.e[e];
+    }
   }
 }
 
@@ -118,7 +178,7 @@ void check_logits_adjust(const KuHipLogitsArgs& a) {
   if (a.rows && overlap(a.logits, ni, a.out, no))
     require(a.logits == a.out && a.dtype == a.out_dtype && (a.rows == 1 || a.logits_stride == a.out_stride),
             "out overlaps logits without being the same");
-  require(a.history <= 0x7fffffff, "history is more than 2^31 - 1");
+  require(a.history <= kCount, "history is more than 2^30 - 1");
   if (a.tokens) span_of((int64_t)a.history, {{a.rows, a.tokens_stride}}, "tokens");
   require(a.tokens || !(a.lens || a.prompt_lens), "lens or prompt_lens without tokens");
   require((a.bias_ids != nullptr) == (a.bias_values != nullptr) && (a.bias_ids != nullptr) == (a.bias_offsets != nullptr),
