@@ -59,9 +59,9 @@ struct SdpaPlan {
   // [0] the prefix with the rows of all sequences (joint: prefix and own keys of a sequence's rows);
   // [1] a sequence's own keys with its rows
   struct Part {
-    bool shared = false;  // four waves of 32 rows share the keys' blocks; else each wave is by itself
+    bool shared = false;  // four waves of 32 rows over the same blocks of keys; else 32 rows, the blocks dealt to the waves
     int tiles = 0, splits = 0;   // row tiles a kv head (and sequence), splits of their keys
-    int units = 0, groups = 0;   // tiles times splits of all of them, and work-groups: one unit each, or one a wave
+    int units = 0;               // work-groups: tiles times splits of all of them
   } part[2];
   int slots = 0;  // partial results a row
 };
@@ -252,36 +252,62 @@ struct Rows {
 template <int DT, int D>
 struct Keys {
   using T = Tile<DT, D>;
-  const char *k, *v;   // row 0 of the head
-  int64_t stride;      // bytes a row
-  int n;               // keys that there are
+  static constexpr int RPD = 1024 / T::RB;  // rows of one DMA instruction
+  const char *k, *v;     // row 0 of the head
+  int64_t stride;        // bytes a row
+  int n;                 // keys that there are
   const int32_t* table;  // pages, or null
   int shift, npages;
-  bool none = false;   // a page that is none was met
+  int held = -1;         // pages held .. held + 63 of the table lie in `page`, one a lane: the loop over
+  int page = 0;          // the blocks then loads nothing that the compiler would wait for
+  bool none = false;     // a page that is none was met
 
-  // byte offset of key j's row
-  __device__ __forceinline__ int64_t offset(int j) {
-    j = j < n ? j : n - 1;
-    if (!table) return j * stride;
-    int32_t page = table[j >> shift];
-    if (page < 0 || page >= npages) {
-      none = true;
-      page = 0;
+  // Byte offsets of the rows that this wave's share (of WAVES) of KEYS keys from j0 on reads.
+  template <int KEYS, int WAVES>
+  __device__ __forceinline__ void rows(int j0, int wave, int64_t (&off)[KEYS / RPD / WAVES]) {
+    constexpr int N = KEYS / RPD / WAVES;
+    static_assert(N * RPD * WAVES == KEYS, "whole DMA instructions");
+    const int lane = threadIdx.x & 63, r = lane / T::CPR;
+    if (table) {
+      const int p0 = j0 >> shift, p1 = (j0 + KEYS - 1 < n ? j0 + KEYS - 1 : n - 1) >> shift;
+      if (held < 0 || p1 >= held + 64) {
+        held = p0;
+        const int last = (n - 1) >> shift;
+        page = table[p0 + lane < last ? p0 + lane : last];
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        int j = j0 + (i * WAVES + wave) * RPD + r;
+        j = j < n ? j : n - 1;
+        int pg = __builtin_amdgcn_ds_bpermute(((j >> shift) - held) << 2, page);
+        if (pg < 0 || pg >= npages) {
+          none = true;
+          pg = 0;
+        }
+        off[i] = (((int64_t)pg << shift) + (j & ((1 << shift) - 1))) * stride;
+      }
+    } else if (j0 + KEYS <= n) {
+      const int64_t mine = r * stride;
+#pragma unroll
+      for (int i = 0; i < N; ++i) off[i] = mine + (int64_t)(j0 + (i * WAVES + wave) * RPD) * stride;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = j0 + (i * WAVES + wave) * RPD + r;
+        off[i] = (int64_t)(j < n ? j : n - 1) * stride;
+      }
     }
-    return (((int64_t)page << shift) + (j & ((1 << shift) - 1))) * stride;
   }
-  // This wave's share (of `waves`) of the DMA of `keys` keys from key j0 into K and V tiles.
-  template <bool V, int KEYS, int WAVES>
-  __device__ __forceinline__ void load(int j0, KU_LDS unsigned char* dst, int wave, int dim) {
-    constexpr int N = KEYS * T::RB / 1024 / WAVES;
-    static_assert(N * WAVES * 1024 == KEYS * T::RB, "whole DMA pieces");
+  // the DMA of those rows of K or V into tiles at dst
+  template <bool V, int N, int WAVES>
+  __device__ __forceinline__ void load(const int64_t (&off)[N], KU_LDS unsigned char* dst, int wave, int dim) const {
     const int lane = threadIdx.x & 63, last = dim * T::ES / 16 - 1;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int blk = i * WAVES + wave, r = blk * (1024 / T::RB) + lane / T::CPR;
+      const int blk = i * WAVES + wave, r = blk * RPD + lane / T::CPR;
       int c = (lane % T::CPR) ^ (V ? T::vswz(r) : T::kswz(r));
       c = c < last ? c : last;  // features past head_dim meet zeros of Q, or are not stored
-      lds_dma16_g((V ? v : k) + offset(j0 + r) + c * 16, (KU_LDS void*)(dst + blk * 1024));
+      lds_dma16_g((V ? v : k) + off[i] + c * 16, (KU_LDS void*)(dst + blk * 1024));
     }
   }
 };
@@ -301,132 +327,118 @@ __device__ __forceinline__ Keys<DT, D> own_keys(const SdpaDev& a, int b, int kvh
           a.page_shift < 0 ? 0 : a.page_shift, a.npages};
 }
 
-// Writes a wave's rows: `row` is this lane's (b, t, h) index or -1. With one slot a row the output
-// itself, else the partial result `slot`.
-template <int DT, int D>
-__device__ __forceinline__ void finish(const SdpaArgs& g, Rows<DT, D>& R, int64_t row, int slot, bool none, float* lds) {
-  using T = Tile<DT, D>;
-  const SdpaDev& a = g.a;
-  const int lane = threadIdx.x & 63, h = lane >> 5;
-  float l = R.l + other_half(R.l);
-  if (none) l = NAN;
-  if (g.p.slots > 1) {
-    if (row < 0) return;
-    float* o = g.po + (row * g.p.slots + slot) * D;
-#pragma unroll
-    for (int t = 0; t < T::DTL; ++t)
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        *reinterpret_cast<f32x4*>(o + 32 * t + 8 * v + 4 * h) =
-            f32x4{R.o[t][4 * v], R.o[t][4 * v + 1], R.o[t][4 * v + 2], R.o[t][4 * v + 3]};
-    if (h == 0) g.ml[row * g.p.slots + slot] = make_float2(R.m, l);
-    return;
-  }
-  // 0 * x is not 0 for a sum that is not finite
-  float z = l * 0.f;
-#pragma unroll
-  for (int t = 0; t < T::DTL; ++t)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) z = fmaf(R.o[t][v], 0.f, z);
-  z += other_half(z);
-  const bool bad = row >= 0 && (!(z == 0.f) || l == 0.f);
-  if (row >= 0 && !bad) {
-    const int64_t tok = row / a.q_heads;
-    const int b = (int)(tok / a.q_len), t0 = (int)(tok % a.q_len), head = (int)(row % a.q_heads);
-    using E = typename SdpaElem<DT>::T;
-    E* out = static_cast<E*>(a.o) + b * a.ob + t0 * a.ot + head * a.oh;
-    const float inv = 1.f / l;
-#pragma unroll
-    for (int t = 0; t < T::DTL; ++t)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int d = 32 * t + 8 * v + 4 * h;
-        if (d >= a.dim) continue;
-        const float x[4] = {R.o[t][4 * v] * inv, R.o[t][4 * v + 1] * inv, R.o[t][4 * v + 2] * inv, R.o[t][4 * v + 3] * inv};
-        if constexpr (DT == GT_F32)
-          *reinterpret_cast<f32x4*>(out + d) = f32x4{x[0], x[1], x[2], x[3]};
-        else
-          *reinterpret_cast<u32x2*>(out + d) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
-      }
-    if (a.lse && h == 0) a.lse[row] = (R.m + __builtin_amdgcn_logf(l)) * LN2;
-  }
-  uint32_t redo = (uint32_t)__builtin_amdgcn_ballot_w64(bad && h == 0);
-  while (redo) {
-    const int i = __builtin_ctz(redo);
-    redo &= redo - 1;
-    const int64_t r = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), i) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, i);
-    sdpa_one<DT>(a, (int)(r / a.q_heads / a.q_len), (int)(r / a.q_heads % a.q_len), (int)(r % a.q_heads), lds);
-  }
-}
-
 // blocks [first, last) of n that split i of s takes
 __device__ __forceinline__ void split_range(int n, int i, int s, int& first, int& last) {
   first = (int)((int64_t)n * i / s);
   last = (int)((int64_t)n * (i + 1) / s);
 }
 
+// Item i of n in an order that gives each XCD (work-groups go to them in turn) a run of items: the row
+// tiles of one split of keys, which come one after another, then read it from one L2.
+__device__ __forceinline__ int xcd_order(int i, int n) {
+  const int x = i & 7, q = n >> 3, r = n & 7;
+  return x * q + (x < r ? x : r) + (i >> 3);
+}
+
+// where a query's row lies
+struct RowAt {
+  int b, t, h;
+  __device__ __forceinline__ RowAt(const SdpaDev& a, int64_t row) {
+    const int64_t tok = row / a.q_heads;
+    b = (int)(tok / a.q_len), t = (int)(tok % a.q_len), h = (int)(row % a.q_heads);
+  }
+};
+
+// four consecutive features from d on of a query's output, normalised
+template <int DT>
+__device__ __forceinline__ void write_out(const SdpaDev& a, const RowAt& at, int d, f32x4 x) {
+  using E = typename SdpaElem<DT>::T;
+  if (d >= a.dim) return;
+  E* out = static_cast<E*>(a.o) + at.b * a.ob + at.t * a.ot + at.h * a.oh + d;
+  if constexpr (DT == GT_F32)
+    *reinterpret_cast<f32x4*>(out) = x;
+  else
+    *reinterpret_cast<u32x2*>(out) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+}
+
+// not finite: 0 * x is not 0
+__device__ __forceinline__ bool bad_sum(float x) { return !(x * 0.f == 0.f); }
+
 template <int DT, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) sdpa_tiles_k(SdpaArgs g) {
   using T = Tile<DT, D>;
   using E = typename SdpaElem<DT>::T;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[T::LDS];
+  __shared__ float2 wave_ml[4][32];
+  __shared__ uint32_t redo_rows, met_none;
   KU_LDS unsigned char* lds = (KU_LDS unsigned char*)lds_raw;
   const SdpaDev& a = g.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const float c = a.scale * LOG2E;
   int id = blockIdx.x;
-  const bool second = id >= g.p.part[0].groups;
+  const bool second = id >= g.p.part[0].units;
   const SdpaPlan::Part& part = g.p.part[second];
-  if (second) id -= g.p.part[0].groups;
-  const bool pooled = !g.p.joint && !second;
+  id = second ? xcd_order(id - g.p.part[0].units, part.units) : xcd_order(id, part.units);
+  const bool pooled = !g.p.joint && !second, shared = part.shared;
 
-  // the work-group's (sequence,) kv head, row tile and split
-  if (!part.shared) id = id * 4 + wave;
-  if (id >= part.units) return;  // all waves of a shared unit, or one by itself
+  // the work-group's (sequence,) kv head, row tile and split of the keys
   const int tile = id % part.tiles;
   id /= part.tiles;
   const int split = id % part.splits;
   id /= part.splits;
   const int kvh = id % a.kv_heads, b = id / a.kv_heads;
   const int per_seq = a.q_len * a.group, nrows = pooled ? a.batch * per_seq : per_seq;
-  const int r = tile * (part.shared ? 128 : 32) + (part.shared ? wave * 32 : 0) + (lane & 31);
+  const int row0 = tile * (shared ? 128 : 32) + (shared ? wave * 32 : 0);  // of this wave
+  const int own_len = pooled ? 0 : sdpa_len(a, b);
+  // (b, t, h) index of row r of the tile's kv head (and sequence)
+  auto row_of = [&](int r) {
+    const int seq = pooled ? r / per_seq : b, in = pooled ? r % per_seq : r;
+    return ((int64_t)seq * a.q_len + in / a.group) * a.q_heads + kvh * a.group + in % a.group;
+  };
   Rows<DT, D> R;
   int64_t row = -1;
   const E* qrow = nullptr;
   R.limit = 0;
-  if (r < nrows) {
-    const int seq = pooled ? r / per_seq : b, in = pooled ? r % per_seq : r, t = in / a.group, head = kvh * a.group + in % a.group;
-    row = ((int64_t)seq * a.q_len + t) * a.q_heads + head;
-    qrow = static_cast<const E*>(a.q) + seq * a.qb + t * a.qt + head * a.qh;
-    if (!pooled) R.limit = sdpa_len(a, b) - (a.q_len - 1 - t);
+  if (row0 + (lane & 31) < nrows) {
+    row = row_of(row0 + (lane & 31));
+    const RowAt at(a, row);
+    qrow = static_cast<const E*>(a.q) + at.b * a.qb + at.t * a.qt + at.h * a.qh;
+    R.limit = own_len - (a.q_len - 1 - at.t);
   }
   R.load_q(qrow, a.dim);
   R.clear();
+  if (threadIdx.x == 0) redo_rows = met_none = 0;
+  __syncthreads();
 
-  bool none = false;
   // the tile's blocks: those of the prefix, then those of the sequence's own keys that its last row sees
-  const int bk = part.shared ? 32 * T::SB : 32;
-  const bool walks_own = second || g.p.joint;
+  const int bk = shared ? 32 * T::SB : 32;
   int own_n = 0;
-  if (walks_own && a.own_max) {
-    const int last_row = std::min(tile * (part.shared ? 128 : 32) + (part.shared ? 127 : 31), nrows - 1);
-    own_n = std::max(0, sdpa_len(a, b) - (a.q_len - 1 - last_row / a.group));
+  if (own_len) {
+    const int last_row = std::min((tile + 1) * (shared ? 128 : 32), nrows) - 1;
+    own_n = std::max(0, own_len - (a.q_len - 1 - last_row / a.group));
   }
   const int np = second ? 0 : (a.prefix + bk - 1) / bk, no = (own_n + bk - 1) / bk;
   int first, last;
   split_range(np + no, split, part.splits, first, last);
-  Keys<DT, D> P = prefix_keys<DT, D>(a, kvh), O = own_keys<DT, D>(a, walks_own ? b : 0, kvh);
-  if (!a.own_max) O.n = 0;
+  Keys<DT, D> P = prefix_keys<DT, D>(a, kvh), O = own_keys<DT, D>(a, b, kvh);
+  O.n = own_len;
 
-  if (part.shared) {
-    constexpr int BK = 32 * T::SB, TB = T::SB * T::KT;
+  if (shared) {
+    // Four waves of 32 rows over blocks of BK keys; the next block's DMA runs under this one's products.
+    constexpr int BK = 32 * T::SB, TB = T::SB * T::KT, N = BK / Keys<DT, D>::RPD / 4;
     auto kbuf = [&](int i) { return lds + i * TB; };
     auto vbuf = [&](int i) { return lds + (2 + i) * TB; };
     auto fetch = [&](int blk) {
-      Keys<DT, D>& S = blk < np ? P : O;
-      const int j0 = (blk < np ? blk : blk - np) * BK;
-      S.template load<false, BK, 4>(j0, kbuf(blk & 1), wave, a.dim);
-      S.template load<true, BK, 4>(j0, vbuf(blk & 1), wave, a.dim);
+      int64_t off[N];
+      if (blk < np) {
+        P.template rows<BK, 4>(blk * BK, wave, off);
+        P.template load<false, N, 4>(off, kbuf(blk & 1), wave, a.dim);
+        P.template load<true, N, 4>(off, vbuf(blk & 1), wave, a.dim);
+      } else {
+        O.template rows<BK, 4>((blk - np) * BK, wave, off);
+        O.template load<false, N, 4>(off, kbuf(blk & 1), wave, a.dim);
+        O.template load<true, N, 4>(off, vbuf(blk & 1), wave, a.dim);
+      }
     };
     if (first < last) fetch(first);
     for (int blk = first; blk < last; ++blk) {
@@ -446,41 +458,150 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
       for (int t = 0; t < T::SB; ++t) R.weigh(s[t], c, vbuf(blk & 1) + t * T::KT);
     }
-    __syncthreads();
   } else {
+    // The waves take blocks of 32 keys in turn, each by itself: K of its next block is fetched once this
+    // one's scores are done, V once its products are, so either is on its way while the other is used.
+    constexpr int N = 32 / Keys<DT, D>::RPD;
     KU_LDS unsigned char *K = lds + wave * 2 * T::KT, *V = K + T::KT;
-    for (int blk = first; blk < last; ++blk) {
-      const bool pre = blk < np;
+    int64_t off[N];
+    auto rows = [&](int blk) {
+      if (blk < np)
+        P.template rows<32, 1>(blk * 32, 0, off);
+      else
+        O.template rows<32, 1>((blk - np) * 32, 0, off);
+    };
+    auto fetch_k = [&](int blk) { blk < np ? P.template load<false, N, 1>(off, K, 0, a.dim) : O.template load<false, N, 1>(off, K, 0, a.dim); };
+    auto fetch_v = [&](int blk) { blk < np ? P.template load<true, N, 1>(off, V, 0, a.dim) : O.template load<true, N, 1>(off, V, 0, a.dim); };
+    int blk = first + wave;
+    if (blk < last) {
+      rows(blk);
+      fetch_k(blk);
+      fetch_v(blk);
+    }
+    for (; blk < last; blk += 4) {
+      const bool pre = blk < np, more = blk + 4 < last;
       const int j0 = (pre ? blk : blk - np) * 32;
-      Keys<DT, D>& S = pre ? P : O;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      S.template load<false, 32, 1>(j0, K, 0, a.dim);
-      S.template load<true, 32, 1>(j0, V, 0, a.dim);
-      vm_wait<0>();
+      vm_wait<N>();  // K is there, V on its way
       asm volatile("" ::: "memory");
       f32x16 s[1];
       s[0] = R.scores(K);
+      if (more) {
+        rows(blk + 4);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+        fetch_k(blk + 4);
+      }
       const int lim = pre ? a.prefix : R.limit;
       if (!pre || j0 + 32 > a.prefix) R.mask(s[0], lim - j0);
       R.rescale(s, c);
+      if (more)
+        vm_wait<N>();
+      else
+        vm_wait<0>();
+      asm volatile("" ::: "memory");
       R.weigh(s[0], c, V);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) fetch_v(blk + 4);
     }
   }
-  none = __builtin_amdgcn_ballot_w64(O.none) != 0;
-  if (part.shared && O.table) {  // any wave of the group may have met it
-    int* flag = reinterpret_cast<int*>(lds_raw);
-    if (threadIdx.x == 0) *flag = 0;
+
+  // ---- the results ----
+  const int slots = g.p.slots, slot = second ? g.p.part[0].splits + split : split;
+  R.l += other_half(R.l);
+  if (__builtin_amdgcn_ballot_w64(O.none) != 0 && lane == 0) atomicOr(&met_none, 1u);
+  uint32_t redo = 0;  // rows of this wave that are done again
+  __syncthreads();
+  if (met_none) R.l = NAN;
+  if (shared) {
+    if (slots > 1) {
+      if (row >= 0) {
+        float* o = g.po + (row * slots + slot) * D;
+#pragma unroll
+        for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            *reinterpret_cast<f32x4*>(o + 32 * t + 8 * v + 4 * h) =
+                f32x4{R.o[t][4 * v], R.o[t][4 * v + 1], R.o[t][4 * v + 2], R.o[t][4 * v + 3]};
+        if (h == 0) g.ml[row * slots + slot] = make_float2(R.m, R.l);
+      }
+    } else {
+      float z = R.l * 0.f;
+#pragma unroll
+      for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) z = fmaf(R.o[t][v], 0.f, z);
+      z += other_half(z);
+      const bool bad = row >= 0 && (!(z == 0.f) || R.l == 0.f);
+      if (row >= 0 && !bad) {
+        const RowAt at(a, row);
+        const float inv = 1.f / R.l;
+#pragma unroll
+        for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            write_out<DT>(a, at, 32 * t + 8 * v + 4 * h,
+                          f32x4{R.o[t][4 * v] * inv, R.o[t][4 * v + 1] * inv, R.o[t][4 * v + 2] * inv, R.o[t][4 * v + 3] * inv});
+        if (a.lse && h == 0) a.lse[row] = (R.m + __builtin_amdgcn_logf(R.l)) * LN2;
+      }
+      redo = (uint32_t)__builtin_amdgcn_ballot_w64(bad && h == 0);
+    }
+  } else {
+    // the waves' results of the same 32 rows are brought to one maximum and added through LDS
+    if (h == 0) wave_ml[wave][lane] = make_float2(R.m, R.l);
     __syncthreads();
-    if (none && lane == 0) atomicOr(flag, 1);
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, wave_ml[w][lane & 31].x);
+    const float from = m == -INFINITY ? 0.f : m;  // nothing seen
+#pragma unroll
+    for (int w = 0; w < 4; ++w) l = fmaf(__builtin_amdgcn_exp2f(wave_ml[w][lane & 31].x - from), wave_ml[w][lane & 31].y, l);
+    const float mine = __builtin_amdgcn_exp2f(R.m - from);
+    if (met_none) l = NAN;
+    constexpr int CH = D / 4;  // 16-byte chunks of a row, swizzled by the row
+    if (row >= 0) {
+      KU_LDS unsigned char* o = lds + wave * 32 * D * 4 + (lane & 31) * D * 4;
+#pragma unroll
+      for (int t = 0; t < T::DTL; ++t)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          *(KU_LDS f32x4*)(o + (((8 * t + 2 * v + h) ^ (lane & (CH - 1) & 31)) << 4)) =
+              f32x4{R.o[t][4 * v] * mine, R.o[t][4 * v + 1] * mine, R.o[t][4 * v + 2] * mine, R.o[t][4 * v + 3] * mine};
+    }
     __syncthreads();
-    none = *flag != 0;
+    if (wave == 0 && h == 0) wave_ml[0][lane] = make_float2(m, l);
     __syncthreads();
+    const int rows = std::min(32, nrows - row0);
+    for (int i = threadIdx.x; i < rows * CH; i += 256) {
+      const int r = i / CH, ch = i % CH;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) o += *(const KU_LDS f32x4*)(lds + w * 32 * D * 4 + r * D * 4 + ((ch ^ (r & (CH - 1) & 31)) << 4));
+      const float2 x = wave_ml[0][r];
+      const int64_t at = row_of(row0 + r);
+      if (slots > 1) {
+        *reinterpret_cast<f32x4*>(g.po + (at * slots + slot) * D + ch * 4) = o;
+        if (ch == 0) g.ml[at * slots + slot] = x;
+      } else {
+        if (bad_sum(x.y) || x.y == 0.f || bad_sum(o[0]) || bad_sum(o[1]) || bad_sum(o[2]) || bad_sum(o[3])) atomicOr(&redo_rows, 1u << r);
+        const float inv = 1.f / x.y;
+        write_out<DT>(a, RowAt(a, at), ch * 4, o * inv);
+        if (ch == 0 && a.lse) a.lse[at] = (x.x + __builtin_amdgcn_logf(x.y)) * LN2;
+      }
+    }
+    if (slots == 1) {
+      __syncthreads();  // also orders the outputs written so far before those written again
+      redo = __builtin_amdgcn_readfirstlane(redo_rows) & (0x11111111u << wave);
+    }
   }
-  finish<DT, D>(g, R, row, second ? g.p.part[0].splits + split : split, none,
-                reinterpret_cast<float*>(lds_raw + wave * 2 * T::KT));
+  while (redo) {
+    const int i = __builtin_ctz(redo);
+    redo &= redo - 1;
+    const RowAt at(a, row_of(row0 + i));
+    sdpa_one<DT>(a, at.b, at.t, at.h, reinterpret_cast<float*>(lds_raw + wave * 2 * T::KT));
+  }
 }
 
-// Joins the partial results of a row, one wave a row.
+// Joins the partial results of a row, one wave a row: the slots' weights in the lanes, then eight slots'
+// outputs at a time.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
   __shared__ float lds[4][kSdpaMaxDim];
@@ -488,39 +609,51 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= (int64_t)a.batch * a.q_len * a.q_heads) return;
-  const float2* ml = g.ml + row * g.p.slots;
   const int n = g.p.slots;
+  const float2* ml = g.ml + row * n;
+  constexpr int L = D / 4, S = 64 / L;  // lanes a slot's output takes, slots side by side
+  const int ch = lane % L, sub = lane / L;
   float m = -INFINITY;
   for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[i].x);
 #pragma unroll
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  constexpr int C = D / 32 < 2 ? 1 : D / 64;  // values a lane
-  float l = 0.f, acc[C] = {};
-  for (int i = 0; i < n; ++i) {
-    const float2 x = ml[i];
-    if (x.x == -INFINITY && x.y == 0.f) continue;  // saw nothing: its output was not summed
-    const float w = __builtin_amdgcn_exp2f(x.x - m);
-    l = fmaf(w, x.y, l);
-    const float* o = g.po + (row * n + i) * D + lane * C;
-    if (D >= 64 || lane < 32)
+  const float from = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const f32x4* po = reinterpret_cast<const f32x4*>(g.po + row * n * D) + ch;
+  for (int i0 = 0; i0 < n; i0 += 8 * S) {
+    f32x4 x[8];
+    float2 y[8];
 #pragma unroll
-      for (int k = 0; k < C; ++k) acc[k] = fmaf(w, o[k], acc[k]);
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * S + sub;
+      x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      y[j] = make_float2(-INFINITY, 0.f);
+      if (i < n) {
+        x[j] = po[(int64_t)i * L];
+        y[j] = ml[i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float w = __builtin_amdgcn_exp2f(y[j].x - from);  // 0 for a slot that saw nothing
+      l = fmaf(w, y[j].y, l);
+      acc += x[j] * w;
+    }
   }
-  float z = l * 0.f;
+  // the slots side by side are added in one order in every lane
 #pragma unroll
-  for (int k = 0; k < C; ++k) z = fmaf(acc[k], 0.f, z);
-  const int64_t tok = row / a.q_heads;
-  const int b = (int)(tok / a.q_len), t = (int)(tok % a.q_len), head = (int)(row % a.q_heads);
-  if (__builtin_amdgcn_ballot_w64(!(z == 0.f)) != 0 || l == 0.f) {
-    sdpa_one<DT>(a, b, t, head, lds[wave]);
+  for (int o = L; o < 64; o <<= 1) {
+    l += __shfl_xor(l, o, 64);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] += __shfl_xor(acc[k], o, 64);
+  }
+  const RowAt at(a, row);
+  if (__builtin_amdgcn_ballot_w64(bad_sum(l) || bad_sum(acc[0]) || bad_sum(acc[1]) || bad_sum(acc[2]) || bad_sum(acc[3])) != 0 || l == 0.f) {
+    sdpa_one<DT>(a, at.b, at.t, at.h, lds[wave]);
     return;
   }
-  using E = typename SdpaElem<DT>::T;
-  E* out = static_cast<E*>(a.o) + b * a.ob + t * a.ot + head * a.oh;
-  const float inv = 1.f / l;
-#pragma unroll
-  for (int k = 0; k < C; ++k)
-    if (lane * C + k < a.dim) out[lane * C + k] = store_elem<DT, E>(acc[k] * inv);
+  if (sub == 0) write_out<DT>(a, at, ch * 4, acc * (1.f / l));
   if (a.lse && lane == 0) a.lse[row] = (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
@@ -574,11 +707,10 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     if (keys == 0 || items == 0 || rows == 0) return;
     part.shared = rows > 32;
     part.tiles = (int)((rows + (part.shared ? 127 : 31)) / (part.shared ? 128 : 32));
-    const int64_t blocks = (keys + (part.shared ? bk_shared : 32) - 1) / (part.shared ? bk_shared : 32);
-    const int64_t want = (part.shared ? 2 : 8) * (int64_t)cu_count();  // work-groups, or waves
+    const int64_t blocks = (keys + (part.shared ? bk_shared : 128) - 1) / (part.shared ? bk_shared : 128);
+    const int64_t want = 2 * (int64_t)cu_count();
     part.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / (items * part.tiles), (blocks + 1) / 2, 256}));
     part.units = (int)(items * part.tiles * part.splits);
-    part.groups = part.shared ? part.units : (part.units + 3) / 4;
   };
   if (p.joint) {
     cut(p.part[0], per_seq, nb * kv, (int64_t)(a.prefix_len + a.own_max));
@@ -594,7 +726,7 @@ int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 template <int DT, int D>
 void launch_d(const SdpaArgs& g, hipStream_t s) {
-  const unsigned groups = (unsigned)(g.p.part[0].groups + g.p.part[1].groups);
+  const unsigned groups = (unsigned)(g.p.part[0].units + g.p.part[1].units);
   if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D>), dim3(groups), dim3(256), 0, s, g);
   const int64_t rows = (int64_t)g.a.batch * g.a.q_len * g.a.q_heads;
   if (g.p.slots != 1) hipLaunchKernelGGL((sdpa_join_k<DT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, g);
