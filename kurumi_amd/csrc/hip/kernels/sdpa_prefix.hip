@@ -27,6 +27,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "decode.h"
 #include "lds_dma.h"
@@ -53,6 +54,22 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // blocks leave O alone; probabilities reach 2^8 at most before they are normalised.
 constexpr float RESCALE = 8.f;
 
+// Division by a number known at the launch: a product, and one correction.
+struct Div {
+  uint32_t d = 1, m = 0xffffffffu;
+  Div() = default;
+  explicit Div(int64_t by) : d((uint32_t)std::max<int64_t>(by, 1)), m((uint32_t)std::min<uint64_t>(((uint64_t)1 << 32) / d, 0xffffffffu)) {}
+  __device__ __forceinline__ int split(int n, int& rest) const {
+    uint32_t q = __umulhi((uint32_t)n, m), r = (uint32_t)n - q * d;
+    if (r >= d) {
+      ++q;
+      r -= d;
+    }
+    rest = (int)r;
+    return (int)q;
+  }
+};
+
 // How a call is cut into work-groups.
 struct SdpaPlan {
   bool joint = false;
@@ -62,8 +79,10 @@ struct SdpaPlan {
     bool shared = false;  // four waves of 32 rows over the same blocks of keys; else 32 rows, the blocks dealt to the waves
     int tiles = 0, splits = 0;   // row tiles a kv head (and sequence), splits of their keys
     int units = 0;               // work-groups: tiles times splits of all of them
+    Div by_tiles, by_splits;
   } part[2];
   int slots = 0;  // partial results a row
+  Div by_kv, by_group, by_seq, by_q_len, by_heads;  // kv heads; q heads of one; a sequence's rows; its queries; q heads
 };
 
 struct SdpaArgs {
@@ -91,16 +110,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const f32x2 v = {lo, hi};
   if constexpr (DT == GT_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-}
-template <int DT>
-__device__ __forceinline__ float sum2(uint32_t pair, float c) {
-  if constexpr (DT == GT_BF16) {
-    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), one, c, false);
-  } else {
-    const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), one, c, false);
-  }
 }
 // the value of the other half of the wave
 __device__ __forceinline__ float other_half(float x) {
@@ -162,10 +171,14 @@ struct Rows {
   __device__ __forceinline__ f32x16 scores(const KU_LDS unsigned char* K) const {
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     f32x16 s = {};
+    u32x4 k[3];  // fragments two steps ahead
+    auto read = [&](int i) { return *(const KU_LDS u32x4*)(K + r * T::RB + (((2 * i + h) ^ T::kswz(r)) << 4)); };
+    k[0] = read(0);
+    if (T::DS > 1) k[1] = read(1);
 #pragma unroll
     for (int i = 0; i < T::DS; ++i) {
-      const u32x4 k = *(const KU_LDS u32x4*)(K + r * T::RB + (((2 * i + h) ^ T::kswz(r)) << 4));
-      mfma_step<DT>(k, q[i], s);
+      if (i + 2 < T::DS) k[(i + 2) % 3] = read(i + 2);
+      mfma_step<DT>(k[i % 3], q[i], s);
     }
     return s;
   }
@@ -196,7 +209,38 @@ struct Rows {
         for (int v = 0; v < 16; ++v) o[t][v] *= corr;
     }
   }
-  // O^T += V^T P^T over 32 keys; the sum adds the probabilities that the product uses
+  // O^T += V^T P^T over 32 keys of 16-bit values, the fragments of V read a step of 16 keys ahead.
+  // V^T fragments by transposing reads: in each 16-lane group input lane 4 k' + j points at key row k',
+  // dims 4 j.. + 3, and output lane i receives keys 0..3 of dim i; two of them fetch the keys that the
+  // probability registers hold, 16 s + 4 h + 0..3 and those + 8.
+  template <int STEPS>
+  __device__ __forceinline__ void product(const u32x4 (&p)[STEPS], const KU_LDS unsigned char* V) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, g = lane >> 4, c16 = lane & 15;
+    auto read = [&](int st, u32x4 (&f)[T::DTL]) {
+#pragma unroll
+      for (int t = 0; t < T::DTL; ++t) {
+        const int d = t * 32 + (g & 1) * 16 + (c16 & 3) * 4;
+        u32x2 half[2];
+#pragma unroll
+        for (int r2 = 0; r2 < 2; ++r2) {
+          const int kr = 16 * st + 8 * r2 + 4 * h + (c16 >> 2);
+          const KU_LDS unsigned char* a = V + kr * T::RB + (((d >> 3) ^ T::vswz(kr)) << 4) + (d & 7) * 2;
+          half[r2] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((KU_LDS s16x4*)a));
+        }
+        f[t] = u32x4{half[0][0], half[0][1], half[1][0], half[1][1]};
+      }
+    };
+    u32x4 f[2][T::DTL];
+    read(0, f[0]);
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      if (st + 1 < STEPS) read(st + 1, f[(st + 1) & 1]);
+#pragma unroll
+      for (int t = 0; t < T::DTL; ++t) mfma_step<DT>(f[st & 1][t], p[st], o[t]);
+    }
+  }
+  // O^T += V^T P^T over 32 keys. The product takes probabilities rounded to the 16 bits of V, half a step
+  // each (the output's own rounding is one more); their sum, which lse is made of, stays in f32.
   __device__ __forceinline__ void weigh(const f32x16& s, float c, const KU_LDS unsigned char* V) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const float em = m == -INFINITY ? 0.f : -m;  // nothing seen so far: every score is -inf
@@ -222,28 +266,11 @@ struct Rows {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * i], c, em));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], c, em));
         const uint32_t pp = pack2<DT>(p0, p1);
-        rs[i & 1] = sum2<DT>(pp, rs[i & 1]);
+        rs[i & 1] += p0 + p1;
         p[i >> 2][i & 3] = pp;
       }
       l += rs[0] + rs[1];
-      // V^T fragments by transposing reads: in each 16-lane group input lane 4 k' + j points at key
-      // row k', dims 4 j.. + 3, and output lane i receives keys 0..3 of dim i; two of them fetch the
-      // keys that the probability registers hold, 16 s + 4 h + 0..3 and those + 8
-      const int g = lane >> 4, c16 = lane & 15;
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int t = 0; t < T::DTL; ++t) {
-          const int d = t * 32 + (g & 1) * 16 + (c16 & 3) * 4;
-          u32x2 half[2];
-#pragma unroll
-          for (int r2 = 0; r2 < 2; ++r2) {
-            const int kr = 16 * st + 8 * r2 + 4 * h + (c16 >> 2);
-            const KU_LDS unsigned char* a = V + kr * T::RB + (((d >> 3) ^ T::vswz(kr)) << 4) + (d & 7) * 2;
-            half[r2] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((KU_LDS s16x4*)a));
-          }
-          mfma_step<DT>(u32x4{half[0][0], half[0][1], half[1][0], half[1][1]}, p[st], o[t]);
-        }
+      product(p, V);
     }
   }
 };
@@ -258,6 +285,7 @@ struct Keys {
   int n;                 // keys that there are
   const int32_t* table;  // pages, or null
   int shift, npages;
+  bool flat;             // rows one after another, 64 of them within 2 GiB: the DMA takes buffer offsets
   int held = -1;         // pages held .. held + 63 of the table lie in `page`, one a lane: the loop over
   int page = 0;          // the blocks then loads nothing that the compiler would wait for
   bool none = false;     // a page that is none was met
@@ -267,6 +295,7 @@ struct Keys {
   __device__ __forceinline__ void rows(int j0, int wave, int64_t (&off)[KEYS / RPD / WAVES]) {
     constexpr int N = KEYS / RPD / WAVES;
     static_assert(N * RPD * WAVES == KEYS, "whole DMA instructions");
+    if (flat) return;
     const int lane = threadIdx.x & 63, r = lane / T::CPR;
     if (table) {
       const int p0 = j0 >> shift, p1 = (j0 + KEYS - 1 < n ? j0 + KEYS - 1 : n - 1) >> shift;
@@ -286,10 +315,6 @@ struct Keys {
         }
         off[i] = (((int64_t)pg << shift) + (j & ((1 << shift) - 1))) * stride;
       }
-    } else if (j0 + KEYS <= n) {
-      const int64_t mine = r * stride;
-#pragma unroll
-      for (int i = 0; i < N; ++i) off[i] = mine + (int64_t)(j0 + (i * WAVES + wave) * RPD) * stride;
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -298,55 +323,107 @@ struct Keys {
       }
     }
   }
-  // the DMA of those rows of K or V into tiles at dst
-  template <bool V, int N, int WAVES>
-  __device__ __forceinline__ void load(const int64_t (&off)[N], KU_LDS unsigned char* dst, int wave, int dim) const {
+  // This wave's share (of WAVES) of the DMA of KEYS keys of K or V from j0 on into tiles at dst; `off` from
+  // rows(), where the keys are not flat. Features past head_dim repeat its last 16 bytes: they meet zeros
+  // of Q, or are not stored. Flat rows past the last key read as zeros, others repeat it.
+  template <bool V, int KEYS, int WAVES>
+  __device__ __forceinline__ void load(int j0, const int64_t (&off)[KEYS / RPD / WAVES], KU_LDS unsigned char* dst, int wave, int dim) const {
+    constexpr int N = KEYS / RPD / WAVES;
     const int lane = threadIdx.x & 63, last = dim * T::ES / 16 - 1;
+    if (flat) {
+      const int left = n - j0 < KEYS ? n - j0 : KEYS;
+      const uint64_t at = reinterpret_cast<uint64_t>((V ? v : k) + (int64_t)j0 * stride);
+      const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 |
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+      const auto R = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), (short)0,
+                                                       __builtin_amdgcn_readfirstlane(left * (int)stride), 0x00020000);
+      // the wave's first destination, opaque to the optimiser: hoisted, the M0 values of all the DMAs
+      // would stay live in SGPRs across the loop and spill
+      KU_LDS unsigned char* wd = dst + wave * 1024;
+      asm volatile("" : "+s"(wd));
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int blk = i * WAVES + wave, r = blk * RPD + lane / T::CPR;
-      int c = (lane % T::CPR) ^ (V ? T::vswz(r) : T::kswz(r));
-      c = c < last ? c : last;  // features past head_dim meet zeros of Q, or are not stored
-      lds_dma16_g((V ? v : k) + off[i] + c * 16, (KU_LDS void*)(dst + blk * 1024));
+      for (int i = 0; i < N; ++i) {
+        const int r = (i * WAVES + wave) * RPD + lane / T::CPR;
+        int c = (lane % T::CPR) ^ (V ? T::vswz(r) : T::kswz(r));
+        c = c < last ? c : last;
+        lds_dma16(R, (uint32_t)(r * (int)stride + c * 16), 0, (KU_LDS void*)(wd + i * WAVES * 1024));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int blk = i * WAVES + wave, r = blk * RPD + lane / T::CPR;
+        int c = (lane % T::CPR) ^ (V ? T::vswz(r) : T::kswz(r));
+        c = c < last ? c : last;
+        lds_dma16_g((V ? v : k) + off[i] + c * 16, (KU_LDS void*)(dst + blk * 1024));
+      }
     }
   }
 };
 
+// the prefix, or sequence b's own `n` keys
 template <int DT, int D>
-__device__ __forceinline__ Keys<DT, D> prefix_keys(const SdpaDev& a, int kvh) {
+__device__ __forceinline__ Keys<DT, D> keys_of(const SdpaDev& a, bool own, int b, int n, int kvh) {
   using E = typename SdpaElem<DT>::T;
-  return {reinterpret_cast<const char*>(static_cast<const E*>(a.pk) + kvh * a.phead),
-          reinterpret_cast<const char*>(static_cast<const E*>(a.pv) + kvh * a.phead), a.prow * (int)sizeof(E), a.prefix, nullptr, 0, 0};
-}
-template <int DT, int D>
-__device__ __forceinline__ Keys<DT, D> own_keys(const SdpaDev& a, int b, int kvh) {
-  using E = typename SdpaElem<DT>::T;
-  const int64_t base = kvh * a.head + (a.page_shift < 0 ? b * a.seq_rows * a.row : 0);
-  return {reinterpret_cast<const char*>(static_cast<const E*>(a.k) + base), reinterpret_cast<const char*>(static_cast<const E*>(a.v) + base),
-          a.row * (int)sizeof(E), sdpa_len(a, b), a.page_shift < 0 ? nullptr : a.pages + b * a.per_seq,
-          a.page_shift < 0 ? 0 : a.page_shift, a.npages};
+  Keys<DT, D> S;
+  const bool paged = own && a.page_shift >= 0;
+  const int64_t base = kvh * (own ? a.head : a.phead) + (own && !paged ? b * a.seq_rows * a.row : 0);
+  S.k = reinterpret_cast<const char*>(static_cast<const E*>(own ? a.k : a.pk) + base);
+  S.v = reinterpret_cast<const char*>(static_cast<const E*>(own ? a.v : a.pv) + base);
+  S.stride = (own ? a.row : a.prow) * (int)sizeof(E);
+  S.n = own ? n : a.prefix;
+  S.table = paged ? a.pages + b * a.per_seq : nullptr;
+  S.shift = paged ? a.page_shift : 0;
+  S.npages = a.npages;
+  S.flat = !paged && S.stride > 0 && S.stride < (1 << 25);
+  return S;
 }
 
-// blocks [first, last) of n that split i of s takes
-__device__ __forceinline__ void split_range(int n, int i, int s, int& first, int& last) {
-  first = (int)((int64_t)n * i / s);
-  last = (int)((int64_t)n * (i + 1) / s);
+// blocks [first, last) of n that split i takes
+__device__ __forceinline__ void split_range(const Div& splits, int n, int i, int& first, int& last) {
+  int rest;
+  const int each = splits.split(n, rest);
+  first = i * each + std::min(i, rest);
+  last = first + each + (i < rest);
 }
 
-// Item i of n in an order that gives each XCD (work-groups go to them in turn) a run of items: the row
-// tiles of one split of keys, which come one after another, then read it from one L2.
-__device__ __forceinline__ int xcd_order(int i, int n) {
-  const int x = i & 7, q = n >> 3, r = n & 7;
-  return x * q + (x < r ? x : r) + (i >> 3);
+// The unit that work-group i takes: of part `second`, number `unit`; false where it has none.
+//
+// Work-groups go to the eight XCDs in turn, and within one to its CUs in turn. Each XCD gets a run of
+// every part's units (neighbouring units read the same keys, and then from one L2), and takes 32 of one
+// part and 32 of the other by turns, so that a CU holds one of the prefix, which keeps its matrix cores
+// busy, beside one of the sequences' own keys, which keeps its memory busy.
+__device__ __forceinline__ bool unit_of(const SdpaPlan& p, int i, bool& second, int& unit) {
+  const int x = i & 7, n0 = p.part[0].units, n1 = p.part[1].units;
+  int j = i >> 3;
+  const int c0 = (n0 + 7) >> 3, c1 = (n1 + 7) >> 3;
+  // chunks of 32 alternate while both parts have whole ones, then what is left of either
+  const int turns = std::min(c0, c1) / 32;
+  if (j < turns * 64) {
+    second = (j >> 5) & 1;
+    j = (j >> 6) * 32 + (j & 31);
+  } else {
+    j -= turns * 32;
+    second = j >= c0;
+    if (second) j -= c0 - turns * 32;
+  }
+  const int n = second ? n1 : n0, q = n >> 3, r = n & 7;
+  if (j >= q + (x < r)) return false;
+  unit = x * q + (x < r ? x : r) + j;
+  return true;
 }
 
 // where a query's row lies
 struct RowAt {
   int b, t, h;
-  __device__ __forceinline__ RowAt(const SdpaDev& a, int64_t row) {
-    const int64_t tok = row / a.q_heads;
-    b = (int)(tok / a.q_len), t = (int)(tok % a.q_len), h = (int)(row % a.q_heads);
+  // row r of a kv head: of all sequences' rows, or of sequence `seq`
+  __device__ __forceinline__ RowAt(const SdpaPlan& p, bool pooled, int seq, int kvh, int r) : b(seq) {
+    if (pooled) b = p.by_seq.split(r, r);
+    t = p.by_group.split(r, h);
+    h += kvh * (int)p.by_group.d;
   }
+  // its (b, t, h) index, and back
+  __device__ __forceinline__ int64_t index(const SdpaDev& a) const { return ((int64_t)b * a.q_len + t) * a.q_heads + h; }
+  __device__ __forceinline__ RowAt(const SdpaPlan& p, int row) { b = p.by_q_len.split(p.by_heads.split(row, h), t); }
 };
 
 // four consecutive features from d on of a query's output, normalised
@@ -364,156 +441,244 @@ __device__ __forceinline__ void write_out(const SdpaDev& a, const RowAt& at, int
 // not finite: 0 * x is not 0
 __device__ __forceinline__ bool bad_sum(float x) { return !(x * 0.f == 0.f); }
 
-template <int DT, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) sdpa_tiles_k(SdpaArgs g) {
+// Every cache line of the arguments at once: read as they are needed, each line's first read waits for
+// memory by itself.
+template <class Args>
+__device__ __forceinline__ void touch_arguments() {
+  const auto* p = (const uint32_t __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+  uint32_t x[(sizeof(Args) + 63) / 64];
+#pragma unroll
+  for (size_t i = 0; i < sizeof(x) / 4; ++i) x[i] = p[i * 16];
+#pragma unroll
+  for (size_t i = 0; i < sizeof(x) / 4; ++i) asm volatile("" ::"s"(x[i]));
+}
+
+// LDS of a work-group beside the tiles of keys.
+struct SdpaShared {
+  float2 ml[4][32];
+  uint32_t redo, none;
+};
+
+// One unit: a tile of rows against a split of its keys. SHARED: four waves of 32 rows share blocks of
+// keys; else the waves deal the blocks of one tile of 32 rows among them.
+template <int DT, int D, bool SHARED>
+__device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id, unsigned char* lds_raw, SdpaShared& sh) {
   using T = Tile<DT, D>;
   using E = typename SdpaElem<DT>::T;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[T::LDS];
-  __shared__ float2 wave_ml[4][32];
-  __shared__ uint32_t redo_rows, met_none;
+  constexpr int ROWS = SHARED ? 128 : 32;
   KU_LDS unsigned char* lds = (KU_LDS unsigned char*)lds_raw;
   const SdpaDev& a = g.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const float c = a.scale * LOG2E;
-  int id = blockIdx.x;
-  const bool second = id >= g.p.part[0].units;
   const SdpaPlan::Part& part = g.p.part[second];
-  id = second ? xcd_order(id - g.p.part[0].units, part.units) : xcd_order(id, part.units);
-  const bool pooled = !g.p.joint && !second, shared = part.shared;
+  const bool joint = SHARED && g.p.joint, pooled = !joint && !second;
 
   // the work-group's (sequence,) kv head, row tile and split of the keys
-  const int tile = id % part.tiles;
-  id /= part.tiles;
-  const int split = id % part.splits;
-  id /= part.splits;
-  const int kvh = id % a.kv_heads, b = id / a.kv_heads;
+  int tile, kvh, split;
+  id = part.by_tiles.split(id, tile);
+  id = g.p.by_kv.split(id, kvh);  // heads before splits: their rows lie next to each other
+  const int b = part.by_splits.split(id, split);
   const int per_seq = a.q_len * a.group, nrows = pooled ? a.batch * per_seq : per_seq;
-  const int row0 = tile * (shared ? 128 : 32) + (shared ? wave * 32 : 0);  // of this wave
-  const int own_len = pooled ? 0 : sdpa_len(a, b);
-  // (b, t, h) index of row r of the tile's kv head (and sequence)
-  auto row_of = [&](int r) {
-    const int seq = pooled ? r / per_seq : b, in = pooled ? r % per_seq : r;
-    return ((int64_t)seq * a.q_len + in / a.group) * a.q_heads + kvh * a.group + in % a.group;
-  };
-  Rows<DT, D> R;
-  int64_t row = -1;
-  const E* qrow = nullptr;
-  R.limit = 0;
-  if (row0 + (lane & 31) < nrows) {
-    row = row_of(row0 + (lane & 31));
-    const RowAt at(a, row);
-    qrow = static_cast<const E*>(a.q) + at.b * a.qb + at.t * a.qt + at.h * a.qh;
-    R.limit = own_len - (a.q_len - 1 - at.t);
-  }
-  R.load_q(qrow, a.dim);
-  R.clear();
-  if (threadIdx.x == 0) redo_rows = met_none = 0;
-  __syncthreads();
-
+  const int row0 = tile * ROWS + (SHARED ? wave * 32 : 0);  // of this wave
+  const int own_len = pooled ? 0 : __builtin_amdgcn_readfirstlane(sdpa_len(a, b));
   // the tile's blocks: those of the prefix, then those of the sequence's own keys that its last row sees
-  const int bk = shared ? 32 * T::SB : 32;
+  constexpr int bk = SHARED ? 32 * T::SB : 32;
   int own_n = 0;
   if (own_len) {
-    const int last_row = std::min((tile + 1) * (shared ? 128 : 32), nrows) - 1;
-    own_n = std::max(0, own_len - (a.q_len - 1 - last_row / a.group));
+    const int last_row = std::min((tile + 1) * ROWS, nrows) - 1;
+    int rest;
+    own_n = std::max(0, own_len - (a.q_len - 1 - g.p.by_group.split(last_row, rest)));
   }
   const int np = second ? 0 : (a.prefix + bk - 1) / bk, no = (own_n + bk - 1) / bk;
-  int first, last;
-  split_range(np + no, split, part.splits, first, last);
-  Keys<DT, D> P = prefix_keys<DT, D>(a, kvh), O = own_keys<DT, D>(a, b, kvh);
-  O.n = own_len;
-
-  if (shared) {
-    // Four waves of 32 rows over blocks of BK keys; the next block's DMA runs under this one's products.
-    constexpr int BK = 32 * T::SB, TB = T::SB * T::KT, N = BK / Keys<DT, D>::RPD / 4;
-    auto kbuf = [&](int i) { return lds + i * TB; };
-    auto vbuf = [&](int i) { return lds + (2 + i) * TB; };
-    auto fetch = [&](int blk) {
-      int64_t off[N];
-      if (blk < np) {
-        P.template rows<BK, 4>(blk * BK, wave, off);
-        P.template load<false, N, 4>(off, kbuf(blk & 1), wave, a.dim);
-        P.template load<true, N, 4>(off, vbuf(blk & 1), wave, a.dim);
-      } else {
-        O.template rows<BK, 4>((blk - np) * BK, wave, off);
-        O.template load<false, N, 4>(off, kbuf(blk & 1), wave, a.dim);
-        O.template load<true, N, 4>(off, vbuf(blk & 1), wave, a.dim);
-      }
-    };
-    if (first < last) fetch(first);
-    for (int blk = first; blk < last; ++blk) {
-      vm_wait<0>();
-      __syncthreads();
-      if (blk + 1 < last) fetch(blk + 1);
-      const bool pre = blk < np;
-      const int j0 = (pre ? blk : blk - np) * BK;
-      f32x16 s[T::SB];
-#pragma unroll
-      for (int t = 0; t < T::SB; ++t) s[t] = R.scores(kbuf(blk & 1) + t * T::KT);
-      const int lim = pre ? a.prefix : R.limit;
-      if (!pre || j0 + BK > a.prefix)
-#pragma unroll
-        for (int t = 0; t < T::SB; ++t) R.mask(s[t], lim - j0 - 32 * t);
-      R.rescale(s, c);
-#pragma unroll
-      for (int t = 0; t < T::SB; ++t) R.weigh(s[t], c, vbuf(blk & 1) + t * T::KT);
+  int split_first, split_last;
+  split_range(part.by_splits, np + no, split, split_first, split_last);
+  bool none = false;
+  Rows<DT, D> R;
+  R.clear();
+  R.limit = 0;
+  if (threadIdx.x == 0) sh.redo = sh.none = 0;
+  __syncthreads();
+  {
+    const E* q = nullptr;
+    if (row0 + (lane & 31) < nrows) {
+      const RowAt at(g.p, pooled, b, kvh, row0 + (lane & 31));
+      q = static_cast<const E*>(a.q) + at.b * a.qb + at.t * a.qt + at.h * a.qh;
+      R.limit = own_len - (a.q_len - 1 - at.t);
     }
-  } else {
-    // The waves take blocks of 32 keys in turn, each by itself: K of its next block is fetched once this
-    // one's scores are done, V once its products are, so either is on its way while the other is used.
-    constexpr int N = 32 / Keys<DT, D>::RPD;
-    KU_LDS unsigned char *K = lds + wave * 2 * T::KT, *V = K + T::KT;
-    int64_t off[N];
-    auto rows = [&](int blk) {
-      if (blk < np)
-        P.template rows<32, 1>(blk * 32, 0, off);
-      else
-        O.template rows<32, 1>((blk - np) * 32, 0, off);
-    };
-    auto fetch_k = [&](int blk) { blk < np ? P.template load<false, N, 1>(off, K, 0, a.dim) : O.template load<false, N, 1>(off, K, 0, a.dim); };
-    auto fetch_v = [&](int blk) { blk < np ? P.template load<true, N, 1>(off, V, 0, a.dim) : O.template load<true, N, 1>(off, V, 0, a.dim); };
-    int blk = first + wave;
-    if (blk < last) {
-      rows(blk);
-      fetch_k(blk);
-      fetch_v(blk);
-    }
-    for (; blk < last; blk += 4) {
-      const bool pre = blk < np, more = blk + 4 < last;
-      const int j0 = (pre ? blk : blk - np) * 32;
-      vm_wait<N>();  // K is there, V on its way
-      asm volatile("" ::: "memory");
-      f32x16 s[1];
-      s[0] = R.scores(K);
-      if (more) {
-        rows(blk + 4);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
-        fetch_k(blk + 4);
-      }
-      const int lim = pre ? a.prefix : R.limit;
-      if (!pre || j0 + 32 > a.prefix) R.mask(s[0], lim - j0);
-      R.rescale(s, c);
-      if (more)
-        vm_wait<N>();
-      else
-        vm_wait<0>();
-      asm volatile("" ::: "memory");
-      R.weigh(s[0], c, V);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (more) fetch_v(blk + 4);
-    }
+    R.load_q(q, a.dim);
   }
 
+  // one run of keys after another: a joint tile's prefix and own keys, or the part's only ones
+#pragma clang loop unroll(disable)
+  for (int seg = second; seg <= (int)(second || joint); ++seg) {
+    const int first = seg ? std::max(split_first, np) - np : split_first, last = seg ? split_last - np : std::min(split_last, np);
+    if (first >= last) continue;
+    Keys<DT, D> S = keys_of<DT, D>(a, seg, b, own_len, kvh);
+    const int all = seg ? 0 : a.prefix;  // keys that every query sees
+    if constexpr (SHARED) {
+      // Four waves of 32 rows over blocks of BK keys, two buffers for K and two for V.
+      constexpr int BK = 32 * T::SB, TB = T::SB * T::KT, N = BK / Keys<DT, D>::RPD / 4;
+      const bool active = row0 < nrows;  // a wave past the last row only fetches
+      auto kbuf = [&](int i) { return lds + i * TB; };
+      auto vbuf = [&](int i) { return lds + (2 + i) * TB; };
+      auto fetch = [&](int blk, auto is_v, KU_LDS unsigned char* dst) {
+        int64_t off[N];
+        S.template rows<BK, 4>(blk * BK, wave, off);
+        S.template load<decltype(is_v)::value, BK, 4>(blk * BK, off, dst, wave, a.dim);
+      };
+      constexpr std::false_type IsK{};
+      constexpr std::true_type IsV{};
+      // keys that are not there or not seen
+      auto mask = [&](f32x16 (&s)[T::SB], int blk) {
+        if (blk * BK + BK > all)
+#pragma unroll
+          for (int t = 0; t < T::SB; ++t) R.mask(s[t], (seg ? R.limit : all) - blk * BK - 32 * t);
+      };
+      if constexpr (DT == GT_F32) {
+        // a step of f32 products takes longer than a read of LDS or the softmax: nothing to interleave
+        fetch(first, IsK, kbuf(0));
+        fetch(first, IsV, vbuf(0));
+        for (int blk = first; blk < last; ++blk) {
+          const int par = (blk - first) & 1;
+          vm_wait<0>();
+          __syncthreads();
+          if (blk + 1 < last) {
+            fetch(blk + 1, IsK, kbuf(par ^ 1));
+            fetch(blk + 1, IsV, vbuf(par ^ 1));
+          }
+          if (!active) continue;
+          f32x16 s[T::SB];
+#pragma unroll
+          for (int t = 0; t < T::SB; ++t) s[t] = R.scores(kbuf(par) + t * T::KT);
+          mask(s, blk);
+          R.rescale(s, c);
+#pragma unroll
+          for (int t = 0; t < T::SB; ++t) R.weigh(s[t], c, vbuf(par) + t * T::KT);
+        }
+      } else {
+        // K runs one block ahead of V: the products of block blk + 1's scores, which are independent of
+        // block blk's softmax, are issued between its exponentials, each fragment of K read two products
+        // ahead (a scheduling barrier after each group keeps them so). Two blocks a trip, so that the
+        // parity of the buffers is a constant.
+        constexpr int NM = 2 * T::DS, PPM = 16 / NM;
+        static_assert(T::SB == 2 && NM * PPM == 16, "exponential pairs a product");
+        auto step = [&](int blk, f32x16 (&sc)[2], f32x16 (&sn)[2], auto par) __attribute__((always_inline)) {
+          constexpr int PAR = decltype(par)::value;
+          if (blk + 2 < last) fetch(blk + 2, IsK, kbuf(PAR));
+          if (blk + 1 < last) fetch(blk + 1, IsV, vbuf(PAR ^ 1));
+          if (active) {
+            mask(sc, blk);
+            R.rescale(sc, c);
+            const float em = R.m == -INFINITY ? 0.f : -R.m;
+            u32x4 p[4];
+            float rs[2] = {0.f, 0.f};
+            const int r = lane & 31;
+            const KU_LDS unsigned char* LK = kbuf(PAR ^ 1);
+            auto kread = [&](int m) {
+              return *(const KU_LDS u32x4*)(LK + ((m & 1) * 32 + r) * T::RB + (((2 * (m >> 1) + h) ^ T::kswz(r)) << 4));
+            };
+            u32x4 kf[3];
+            kf[0] = kread(0);
+            kf[1] = kread(1);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+              if (m + 2 < NM) kf[(m + 2) % 3] = kread(m + 2);
+#pragma unroll
+              for (int e = 0; e < PPM; ++e) {
+                const int i = m * PPM + e, te = i >> 3, v2 = i & 7;
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2], c, em));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2 + 1], c, em));
+                const uint32_t pp = pack2<DT>(p0, p1);
+                rs[v2 & 1] += p0 + p1;  // unrounded: the sum is an output too
+                p[2 * te + (v2 >> 2)][v2 & 3] = pp;
+              }
+              if (m < 2) sn[m & 1] = f32x16{};
+              mfma_step<DT>(kf[m % 3], R.q[m >> 1], sn[m & 1]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            R.l += rs[0] + rs[1];
+            R.product(p, vbuf(PAR));
+          }
+          vm_wait<0>();
+          __syncthreads();
+        };
+        fetch(first, IsK, kbuf(0));
+        fetch(first, IsV, vbuf(0));
+        if (first + 1 < last) fetch(first + 1, IsK, kbuf(1));
+        vm_wait<0>();
+        __syncthreads();
+        f32x16 sa[2], sb[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) sa[t] = R.scores(kbuf(0) + t * T::KT);
+        __syncthreads();  // every wave has read K's first buffer
+        for (int blk = first; blk < last; blk += 2) {
+          step(blk, sa, sb, std::integral_constant<int, 0>{});
+          if (blk + 1 < last) step(blk + 1, sb, sa, std::integral_constant<int, 1>{});
+        }
+      }
+    } else {
+      // The waves take blocks of 32 keys in turn, each by itself: K of its next block is fetched once this
+      // one's scores are done, V once its products are, so either is on its way while the other is used.
+      constexpr int N = 32 / Keys<DT, D>::RPD;
+      KU_LDS unsigned char *K = lds + wave * 2 * T::KT, *V = K + T::KT;
+      int64_t off[N];
+      auto fetch_k = [&](int blk) {
+        S.template rows<32, 1>(blk * 32, 0, off);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last block's K has been read
+        S.template load<false, 32, 1>(blk * 32, off, K, 0, a.dim);
+      };
+      auto fetch_v = [&](int blk) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        S.template load<true, 32, 1>(blk * 32, off, V, 0, a.dim);
+      };
+      int blk = first + wave;
+      if (blk < last) {
+        fetch_k(blk);
+        fetch_v(blk);
+      }
+      for (; blk < last; blk += 4) {
+        const bool more = blk + 4 < last;
+        vm_wait<N>();  // K is there, V on its way
+        asm volatile("" ::: "memory");
+        f32x16 s[1];
+        s[0] = R.scores(K);
+        if (more) fetch_k(blk + 4);
+        if (blk * 32 + 32 > all) R.mask(s[0], (seg ? R.limit : all) - blk * 32);
+        R.rescale(s, c);
+        if (more)
+          vm_wait<N>();
+        else
+          vm_wait<0>();
+        asm volatile("" ::: "memory");
+        R.weigh(s[0], c, V);
+        if (more) fetch_v(blk + 4);
+      }
+    }
+    none |= S.none;
+  }
+
+  {
   // ---- the results ----
+  // The arguments read afresh: kept across the loop, what only this part uses cost it its registers.
+  const SdpaArgs* afresh = static_cast<const SdpaArgs*>((const void*)__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(afresh));
+  const SdpaArgs& g = *afresh;
+  const SdpaDev& a = g.a;
+  auto at_row = [&](int r) { return RowAt(g.p, pooled, b, kvh, r); };
+  const bool there = row0 + (lane & 31) < nrows;
   const int slots = g.p.slots, slot = second ? g.p.part[0].splits + split : split;
   R.l += other_half(R.l);
-  if (__builtin_amdgcn_ballot_w64(O.none) != 0 && lane == 0) atomicOr(&met_none, 1u);
+  if (__builtin_amdgcn_ballot_w64(none) != 0 && lane == 0) atomicOr(&sh.none, 1u);
   uint32_t redo = 0;  // rows of this wave that are done again
   __syncthreads();
-  if (met_none) R.l = NAN;
-  if (shared) {
+  if (sh.none) R.l = NAN;
+  if constexpr (SHARED) {
+    const RowAt at = at_row(there ? row0 + (lane & 31) : 0);
+    const int64_t row = at.index(a);
     if (slots > 1) {
-      if (row >= 0) {
+      if (there) {
         float* o = g.po + (row * slots + slot) * D;
 #pragma unroll
         for (int t = 0; t < T::DTL; ++t)
@@ -530,9 +695,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int v = 0; v < 16; ++v) z = fmaf(R.o[t][v], 0.f, z);
       z += other_half(z);
-      const bool bad = row >= 0 && (!(z == 0.f) || R.l == 0.f);
-      if (row >= 0 && !bad) {
-        const RowAt at(a, row);
+      const bool bad = there && (!(z == 0.f) || R.l == 0.f);
+      if (there && !bad) {
         const float inv = 1.f / R.l;
 #pragma unroll
         for (int t = 0; t < T::DTL; ++t)
@@ -546,18 +710,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
   } else {
     // the waves' results of the same 32 rows are brought to one maximum and added through LDS
-    if (h == 0) wave_ml[wave][lane] = make_float2(R.m, R.l);
+    if (h == 0) sh.ml[wave][lane] = make_float2(R.m, R.l);
     __syncthreads();
     float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, wave_ml[w][lane & 31].x);
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, sh.ml[w][lane & 31].x);
     const float from = m == -INFINITY ? 0.f : m;  // nothing seen
 #pragma unroll
-    for (int w = 0; w < 4; ++w) l = fmaf(__builtin_amdgcn_exp2f(wave_ml[w][lane & 31].x - from), wave_ml[w][lane & 31].y, l);
+    for (int w = 0; w < 4; ++w) l = fmaf(__builtin_amdgcn_exp2f(sh.ml[w][lane & 31].x - from), sh.ml[w][lane & 31].y, l);
     const float mine = __builtin_amdgcn_exp2f(R.m - from);
-    if (met_none) l = NAN;
+    if (sh.none) l = NAN;
     constexpr int CH = D / 4;  // 16-byte chunks of a row, swizzled by the row
-    if (row >= 0) {
+    if (there) {
       KU_LDS unsigned char* o = lds + wave * 32 * D * 4 + (lane & 31) * D * 4;
 #pragma unroll
       for (int t = 0; t < T::DTL; ++t)
@@ -567,7 +731,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
               f32x4{R.o[t][4 * v] * mine, R.o[t][4 * v + 1] * mine, R.o[t][4 * v + 2] * mine, R.o[t][4 * v + 3] * mine};
     }
     __syncthreads();
-    if (wave == 0 && h == 0) wave_ml[0][lane] = make_float2(m, l);
+    if (wave == 0 && h == 0) sh.ml[0][lane] = make_float2(m, l);
     __syncthreads();
     const int rows = std::min(32, nrows - row0);
     for (int i = threadIdx.x; i < rows * CH; i += 256) {
@@ -575,29 +739,45 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) o += *(const KU_LDS f32x4*)(lds + w * 32 * D * 4 + r * D * 4 + ((ch ^ (r & (CH - 1) & 31)) << 4));
-      const float2 x = wave_ml[0][r];
-      const int64_t at = row_of(row0 + r);
+      const float2 x = sh.ml[0][r];
+      const RowAt where = at_row(row0 + r);
+      const int64_t at = where.index(a);
       if (slots > 1) {
         *reinterpret_cast<f32x4*>(g.po + (at * slots + slot) * D + ch * 4) = o;
         if (ch == 0) g.ml[at * slots + slot] = x;
       } else {
-        if (bad_sum(x.y) || x.y == 0.f || bad_sum(o[0]) || bad_sum(o[1]) || bad_sum(o[2]) || bad_sum(o[3])) atomicOr(&redo_rows, 1u << r);
+        if (bad_sum(x.y) || x.y == 0.f || bad_sum(o[0]) || bad_sum(o[1]) || bad_sum(o[2]) || bad_sum(o[3])) atomicOr(&sh.redo, 1u << r);
         const float inv = 1.f / x.y;
-        write_out<DT>(a, RowAt(a, at), ch * 4, o * inv);
+        write_out<DT>(a, where, ch * 4, o * inv);
         if (ch == 0 && a.lse) a.lse[at] = (x.x + __builtin_amdgcn_logf(x.y)) * LN2;
       }
     }
     if (slots == 1) {
       __syncthreads();  // also orders the outputs written so far before those written again
-      redo = __builtin_amdgcn_readfirstlane(redo_rows) & (0x11111111u << wave);
+      redo = __builtin_amdgcn_readfirstlane(sh.redo) & (0x11111111u << wave);
     }
   }
   while (redo) {
     const int i = __builtin_ctz(redo);
     redo &= redo - 1;
-    const RowAt at(a, row_of(row0 + i));
-    sdpa_one<DT>(a, at.b, at.t, at.h, reinterpret_cast<float*>(lds_raw + wave * 2 * T::KT));
+    const RowAt at = at_row(row0 + i);
+    sdpa_one<DT>(a, at.b, at.t, at.h, reinterpret_cast<float*>(lds_raw + wave * 32 * D * 4));
   }
+  }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) sdpa_tiles_k(SdpaArgs g) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[Tile<DT, D>::LDS];
+  __shared__ SdpaShared sh;
+  touch_arguments<SdpaArgs>();
+  bool second;
+  int unit;
+  if (!unit_of(g.p, blockIdx.x, second, unit)) return;
+  if (g.p.part[second].shared)
+    run_unit<DT, D, true>(g, second, unit, lds, sh);
+  else
+    run_unit<DT, D, false>(g, second, unit, lds, sh);
 }
 
 // Joins the partial results of a row, one wave a row: the slots' weights in the lanes, then eight slots'
@@ -648,7 +828,7 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] += __shfl_xor(acc[k], o, 64);
   }
-  const RowAt at(a, row);
+  const RowAt at(g.p, (int)row);
   if (__builtin_amdgcn_ballot_w64(bad_sum(l) || bad_sum(acc[0]) || bad_sum(acc[1]) || bad_sum(acc[2]) || bad_sum(acc[3])) != 0 || l == 0.f) {
     sdpa_one<DT>(a, at.b, at.t, at.h, lds[wave]);
     return;
@@ -694,31 +874,43 @@ SdpaDev device_args(const KuHipSdpaPrefixArgs& a) {
   return d;
 }
 
-// Whether one sequence's rows fill tiles of 128 well enough to walk the prefix by themselves; where they
-// do not, the sequences' rows share tiles over the prefix.
 SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
   SdpaPlan p;
-  const int64_t per_seq = (int64_t)(a.q_len * (a.q_heads / a.kv_heads)), kv = (int64_t)a.kv_heads, nb = (int64_t)a.batch;
-  const bool f32 = a.dtype == KU_F32;
-  const int64_t bk_shared = f32 ? 32 : 64;
-  const int64_t full = (per_seq + 127) / 128 * 128;
-  p.joint = full * 4 <= per_seq * 5;
-  auto cut = [&](SdpaPlan::Part& part, int64_t rows, int64_t items, int64_t keys) {
+  const int64_t group = (int64_t)(a.q_heads / a.kv_heads), per_seq = (int64_t)a.q_len * group, kv = (int64_t)a.kv_heads,
+                nb = (int64_t)a.batch, cu = cu_count();
+  // One sequence's rows walk the prefix by themselves where they fill tiles of 128 to four fifths; else
+  // the sequences' rows share tiles over it.
+  p.joint = (per_seq + 127) / 128 * 128 * 4 <= per_seq * 5;
+  auto cut = [&](SdpaPlan::Part& part, int64_t rows, int64_t items, int64_t keys, int64_t want) {
     if (keys == 0 || items == 0 || rows == 0) return;
-    part.shared = rows > 32;
+    // Tiles of 128 rows read a key once where four tiles of 32 read it four times (from L2, and with every
+    // wave's own DMA); tiles of 32 spread few rows' keys over all four waves. us of the kernel, bf16, 32
+    // heads over 8 of 128, 8192 shared keys: 48 rows 14.5 / 13.0, 96 rows 27.8 / 25.8 (own keys among
+    // them); 65536 keys: 64 rows 68 / 67, 128 rows 65.6 / 88.9.
+    part.shared = rows > 64;
     part.tiles = (int)((rows + (part.shared ? 127 : 31)) / (part.shared ? 128 : 32));
-    const int64_t blocks = (keys + (part.shared ? bk_shared : 128) - 1) / (part.shared ? bk_shared : 128);
-    const int64_t want = 2 * (int64_t)cu_count();
-    part.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / (items * part.tiles), (blocks + 1) / 2, 256}));
+    const int64_t bk = part.shared ? (a.dtype == KU_F32 ? 32 : 64) : 128, blocks = (keys + bk - 1) / bk;
+    part.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / (items * part.tiles), blocks, 256}));
     part.units = (int)(items * part.tiles * part.splits);
+    part.by_tiles = Div(part.tiles);
+    part.by_splits = Div(part.splits);
   };
   if (p.joint) {
-    cut(p.part[0], per_seq, nb * kv, (int64_t)(a.prefix_len + a.own_max));
+    cut(p.part[0], per_seq, nb * kv, (int64_t)(a.prefix_len + a.own_max), 2 * cu);
   } else {
-    cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len);
-    cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max);
+    // A unit costs about 4 us before its first product and 3 to write its partial result, so more of them
+    // than CUs lose: the prefix alone 22.5 us with one a CU, 28 with two, 31 with one for two CUs (256 rows,
+    // 8192 keys). Beside own keys of half its length or more it leaves every other CU to them: 49 us, and 55
+    // with one a CU (64 sequences of up to 1024 own keys).
+    cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len, nb * (int64_t)a.own_max * 2 >= (int64_t)a.prefix_len ? cu / 2 : cu);
+    cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max, 2 * cu);
   }
   p.slots = p.part[0].splits + p.part[1].splits;
+  p.by_kv = Div(kv);
+  p.by_group = Div(group);
+  p.by_seq = Div(per_seq);
+  p.by_q_len = Div((int64_t)a.q_len);
+  p.by_heads = Div((int64_t)a.q_heads);
   return p;
 }
 
@@ -726,7 +918,7 @@ int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 template <int DT, int D>
 void launch_d(const SdpaArgs& g, hipStream_t s) {
-  const unsigned groups = (unsigned)(g.p.part[0].units + g.p.part[1].units);
+  const unsigned groups = 8 * (unsigned)((g.p.part[0].units + 7) / 8 + (g.p.part[1].units + 7) / 8);
   if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D>), dim3(groups), dim3(256), 0, s, g);
   const int64_t rows = (int64_t)g.a.batch * g.a.q_len * g.a.q_heads;
   if (g.p.slots != 1) hipLaunchKernelGGL((sdpa_join_k<DT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, g);

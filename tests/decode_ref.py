@@ -97,8 +97,9 @@ def sdpa_prefix(q, pk, pv, k, v, lens, scale, *, seq_rows=0, pages=None, page=0,
 
     A score is a dot product of d terms in f32, then scaled: off by at most (d + 2) u sum |q k| scale,
     which moves a probability by as much of itself; exp2 and its argument's rounding, |score| log2 e u,
-    add a few u. The sums over n keys round n times at most. 16-bit probabilities round to half a step
-    (f16 ones to 2^-25 of the largest at least). The output rounds once more."""
+    add a few u. The sums over n keys round n times at most. The probabilities that meet 16-bit values
+    round to half a step (f16 ones to 2^-25 of the largest at least), their sum does not. The output
+    rounds once more."""
     nb, nt, nh, d = q.shape
     kv = pk.shape[1] if pk is not None else k.shape[1]
     g = nh // kv
@@ -124,16 +125,16 @@ def sdpa_prefix(q, pk, pv, k, v, lens, scale, *, seq_rows=0, pages=None, page=0,
                     out[b, t, h] = p @ vv / l
                     lse[b, t, h] = np.nan if np.isnan(s).any() else m + np.log(l) if np.isfinite(m) else m
                     ds = ((d + 2) * U * scale * (np.abs(keys[:, h // g]) @ np.abs(q[b, t, h])) + 4 * U * (np.abs(s) + np.abs(m)) + 8 * U)
-                    rel = ds + (len(keys) + 16) * U + (HALF_STEP[dt] if dt != DType.F32 else 0)
-                    rel = np.where(p > 0, rel, 0.0)  # a score of -inf weighs nothing, whatever its terms
+                    # a score of -inf weighs nothing, whatever its terms
+                    rel = np.where(p > 0, ds + (len(keys) + 16) * U, 0.0)
+                    half = HALF_STEP[dt] if dt != DType.F32 else 0.0
                     # numerator and denominator are off by the same kind of error
-                    e = (p * rel) @ np.abs(vv) / l + (p * rel).sum() / l * np.abs(out[b, t, h])
+                    le = (p * rel).sum() / l
+                    e = (p * (rel + half)) @ np.abs(vv) / l + le * np.abs(out[b, t, h])
                     if dt == DType.F16:
-                        e = e + len(keys) * 2.0 ** -25 * (np.abs(vv).max(0) + np.abs(out[b, t, h])) / l
+                        e = e + len(keys) * 2.0 ** -25 * np.abs(vv).max(0) / l
                     tol[b, t, h] = e + (rounding(out[b, t, h], dt) if dt != DType.F32 else U * np.abs(out[b, t, h]))
-                    ltol[b, t, h] = (p * rel).sum() / l + 4 * U * (np.abs(lse[b, t, h]) + 1)
-                    if dt == DType.F16:
-                        ltol[b, t, h] += len(keys) * 2.0 ** -25 / l
+                    ltol[b, t, h] = le + 4 * U * (np.abs(lse[b, t, h]) + 1)
     return out, lse, np.nan_to_num(tol), np.nan_to_num(ltol)
 
 
