@@ -18,8 +18,9 @@ namespace ku::hipbk {
 
 namespace {
 
-constexpr int kThreads = 512, kVec = 8, kPerThread = 2;  // a thread's logits: two vectors of 8
-constexpr int kChunk = kThreads * kVec * kPerThread;
+constexpr int kThreads = 512;
+constexpr int kLarge = 16, kSmall = 4;  // logits a thread: chunks of 8192 or 2048
+constexpr int kIds = 8;                 // vectors of four token ids a thread has in flight
 // A counter: how often the token was generated, and whether it is in the prompt and has biases.
 constexpr uint32_t kInPrompt = 0x80000000u, kBiased = 0x40000000u, kCount = kBiased - 1;
 
@@ -40,32 +41,34 @@ struct LogitsDev {
 
 __device__ __forceinline__ int32_t clamped(int32_t v, int32_t hi) { return v < 0 ? 0 : v > hi ? hi : v; }
 
-// kVec logits from (to) element alignment: rows of an odd vocabulary start anywhere.
-template <class T>
+// N elements at element alignment: rows of an odd vocabulary start anywhere.
+template <class T, int N>
 struct __attribute__((packed, aligned(sizeof(T)))) Vec {
-  T e[kVec];
+  T e[N];
 };
 
-template <int DT, class T, int OT, class O>
+template <int DT, class T, int OT, class O, int PER>
 __global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
-  __shared__ __attribute__((aligned(16))) uint32_t count[kChunk];
-  __shared__ float bias[kChunk];
+  // what the wider side moves 16 bytes at a time: consecutive lanes then write consecutive pieces
+  constexpr int WIDE = 16 / (int)(sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O)), V = WIDE < PER ? WIDE : PER, N = PER / V;
+  constexpr int CHUNK = kThreads * PER;
+  __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
   __shared__ int repeats;
-  const int64_t r = blockIdx.x / a.chunks, c0 = (int64_t)(blockIdx.x % a.chunks) * kChunk;
-  const int n = (int)(a.vocab - c0 < kChunk ? a.vocab - c0 : kChunk), tid = threadIdx.x;
+  const int64_t r = blockIdx.x / a.chunks, c0 = (int64_t)(blockIdx.x % a.chunks) * CHUNK;
+  const int n = (int)(a.vocab - c0 < CHUNK ? a.vocab - c0 : CHUNK), tid = threadIdx.x;
   const T* x = static_cast<const T*>(a.x) + r * a.xs + c0;
   O* y = static_cast<O*>(a.y) + r * a.ys + c0;
 
   // the logits are on their way while the tokens are counted
-  Vec<T> in[kPerThread];
+  Vec<T, V> in[N];
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) {
-    const int i = (j * kThreads + tid) * kVec;
-    if (i + kVec <= n) {
-      in[j] = *reinterpret_cast<const Vec<T>*>(x + i);
+  for (int j = 0; j < N; ++j) {
+    const int i = (j * kThreads + tid) * V;
+    if (i + V <= n) {
+      in[j] = *reinterpret_cast<const Vec<T, V>*>(x + i);
     } else {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
+      for (int e = 0; e < V; ++e)
         if (i + e < n) in[j].e[e] = x[i + e];
     }
   }
@@ -85,81 +88,124 @@ __global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
     const int64_t m = a.mask_index ? a.mask_index[r] : r;
     if (m >= 0 && m < a.mask_rows) bits = reinterpret_cast<const uint8_t*>(a.mask + m * a.ms) + c0 / 8;
   }
+  uint32_t allowed[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = (j * kThreads + tid) * V;
+    allowed[j] = bits && i < n ? bits[i / 8] >> (i & 7) : 0xffu;
+  }
   const bool counts = len > 0 || e1 > e0;
+  // the place of token v in the chunk, or one past it
+  auto place = [&](int32_t v) {
+    const uint64_t at = (uint64_t)((int64_t)v - c0);
+    return at < (uint64_t)n ? (int)at : CHUNK;
+  };
   if (counts) {
 #pragma unroll
-    for (int i = 0; i < kChunk / 4 / kThreads; ++i) reinterpret_cast<uint4*>(count)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < PER / 4; ++i) reinterpret_cast<uint4*>(count)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
     if (tid == 0) repeats = 0;
     __syncthreads();
     const int32_t* tok = a.tokens + r * a.ts;
-    for (int32_t i0 = 0; i0 < len; i0 += 4 * kThreads) {
-      int32_t id[4];
+    for (int32_t i0 = 0; i0 < len; i0 += 4 * kIds * kThreads) {
+      Vec<int32_t, 4> id[kIds];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) id[j] = i0 + j * kThreads + tid < len ? tok[i0 + j * kThreads + tid] : -1;
+      for (int j = 0; j < kIds; ++j) {
+        const int32_t i = i0 + 4 * (j * kThreads + tid);
+        if (i + 4 <= len) {
+          id[j] = *reinterpret_cast<const Vec<int32_t, 4>*>(tok + i);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t at = (int64_t)id[j] - c0;
-        if (at < 0 || at >= n) continue;
-        if (i0 + j * kThreads + tid < prompt)
-          atomicOr(&count[at], kInPrompt);
-        else
-          atomicAdd(&count[at], 1u);
+          for (int e = 0; e < 4; ++e) id[j].e[e] = i + e < len ? tok[i + e] : -1;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kIds; ++j) {
+        const int32_t i = i0 + 4 * (j * kThreads + tid);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = place(id[j].e[e]);
+          if (at == CHUNK) continue;
+          if (i + e < prompt)
+            atomicOr(&count[at], kInPrompt);
+          else
+            atomicAdd(&count[at], 1u);
+        }
       }
     }
-    // an id of a row's biases comes once as a rule: its bias is put down by the thread that reads it
     for (int32_t e = e0 + tid; e < e1; e += kThreads) {
-      const int64_t at = (int64_t)a.bias_ids[e] - c0;
-      if (at < 0 || at >= n) continue;
-      if (atomicOr(&count[at], kBiased) & kBiased) repeats = 1;
-      bias[at] = a.bias_values[e];
+      const int at = place(a.bias_ids[e]);
+      if (at != CHUNK && (atomicOr(&count[at], kBiased) & kBiased)) repeats = 1;
     }
     __syncthreads();
-    if (repeats) {
-      // some come again: each thread sums those of its places (at % kThreads) in list order
-      for (int i = tid; i < n; i += kThreads) bias[i] = 0.f;
-      for (int32_t e = e0; e < e1; ++e) {
-        const int64_t at = (int64_t)a.bias_ids[e] - c0;
-        if (at >= 0 && at < n && at % kThreads == tid) bias[at] += a.bias_values[e];
-      }
-      __syncthreads();
-    }
   }
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) {
-    const int i = (j * kThreads + tid) * kVec;
+  for (int j = 0; j < N; ++j) {
+    const int i = (j * kThreads + tid) * V;
     if (i >= n) break;
-    const uint32_t allowed = bits ? bits[i / 8] : 0xffu;
-    Vec<O> out;
+    Vec<O, V> out;
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
+    for (int e = 0; e < V; ++e) {
       float v = load_elem<DT, T, float>(in[j].e[e]);
       const uint32_t c = counts ? count[i + e] : 0;
       if (c) {
         const uint32_t g = c & kCount;
         if (c & ~kBiased) v = v > 0.f ? v / rep : v * rep;
         if (g) v -= fmaf(freq, (float)g, pres);
-        if (c & kBiased) v += bias[i + e];
+        if (c & kBiased) count[i + e] = __float_as_uint(v);  // for the bias, below
       }
-      if (!(allowed >> e & 1)) v = -INFINITY;
+      if (!(allowed[j] >> e & 1)) v = -INFINITY;
       out.e[e] = store_elem<OT, O>(v);
     }
-    if (i + kVec <= n) {
-      *reinterpret_cast<Vec<O>*>(y + i) = out;
+    if (i + V <= n) {
+      *reinterpret_cast<Vec<O, V>*>(y + i) = out;
     } else {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
+      for (int e = 0; e < V; ++e)
         if (i + e < n) y[i + e] = out.e[e];
     }
   }
+  if (e1 <= e0) return;
+  // The few biased logits are written again, by the threads that read their biases. An id comes once as a
+  // rule; where one comes again, each thread adds those of its places (at % kThreads) in list order first.
+  __syncthreads();
+  const bool again = repeats;
+  if (again) {
+    for (int32_t e = e0; e < e1; ++e) {
+      const int at = place(a.bias_ids[e]);
+      if (at != CHUNK && at % kThreads == tid) count[at] = __float_as_uint(__uint_as_float(count[at]) + a.bias_values[e]);
+    }
+    __syncthreads();
+  }
+  for (int32_t e = e0 + tid; e < e1; e += kThreads) {
+    const int at = place(a.bias_ids[e]);
+    if (at == CHUNK || (bits && !(bits[at / 8] >> (at & 7) & 1))) continue;
+    const float v = __uint_as_float(count[at]);
+    y[at] = store_elem<OT, O>(again ? v : v + a.bias_values[e]);
+  }
 }
 
-template <int DT, class T>
-void launch_t(const LogitsDev& d, uint32_t out, int64_t rows, hipStream_t s) {
+// Large chunks read a row's tokens fewer times, small ones spread few rows over the chip.
+bool large_chunks(int64_t vocab, int64_t rows) {
+  return (vocab + kThreads * kLarge - 1) / (kThreads * kLarge) * rows >= 2 * (int64_t)cu_count();
+}
+
+template <int DT, class T, int OT, class O>
+void launch_o(LogitsDev& d, int64_t rows, hipStream_t s) {
+  const bool large = large_chunks(d.vocab, rows);
+  const int64_t chunk = kThreads * (large ? kLarge : kSmall);
+  d.chunks = (uint32_t)((d.vocab + chunk - 1) / chunk);
   const dim3 grid((unsigned)(d.chunks * rows));
+  if (large)
+    hipLaunchKernelGGL((logits_k<DT, T, OT, O, kLarge>), grid, dim3(kThreads), 0, s, d);
+  else
+    hipLaunchKernelGGL((logits_k<DT, T, OT, O, kSmall>), grid, dim3(kThreads), 0, s, d);
+}
+template <int DT, class T>
+void launch_t(LogitsDev& d, uint32_t out, int64_t rows, hipStream_t s) {
   switch (out) {
-    case KU_BF16: hipLaunchKernelGGL((logits_k<DT, T, GT_BF16, uint16_t>), grid, dim3(kThreads), 0, s, d); break;
-    case KU_F16: hipLaunchKernelGGL((logits_k<DT, T, GT_F16, uint16_t>), grid, dim3(kThreads), 0, s, d); break;
-    default: hipLaunchKernelGGL((logits_k<DT, T, GT_F32, float>), grid, dim3(kThreads), 0, s, d); break;
+    case KU_BF16: launch_o<DT, T, GT_BF16, uint16_t>(d, rows, s); break;
+    case KU_F16: launch_o<DT, T, GT_F16, uint16_t>(d, rows, s); break;
+    default: launch_o<DT, T, GT_F32, float>(d, rows, s); break;
   }
 }
 
@@ -170,7 +216,7 @@ void check_logits_adjust(const KuHipLogitsArgs& a) {
   const int64_t w = (int64_t)float_width(a.dtype, "dtype"), wo = (int64_t)float_width(a.out_dtype, "out_dtype");
   require(a.rows <= 0x7fffffff, "too many rows");
   require(a.vocab >= 1 && a.vocab <= 0x7fffffff, "vocab must be 1 to 2^31 - 1");
-  require((__int128)((a.vocab + kChunk - 1) / kChunk) * a.rows <= 0x7fffffff, "too many rows of this vocab");
+  require((__int128)((a.vocab + kThreads * kSmall - 1) / (kThreads * kSmall)) * a.rows <= 0x7fffffff, "too many rows of this vocab");
   require((a.logits && a.out) || a.rows == 0, "null logits or out");
   require(aligned_to(a.logits, (size_t)w) && aligned_to(a.out, (size_t)wo), "pointers must be aligned to their elements");
   const int64_t ni = span_of((int64_t)a.vocab, {{a.rows, a.logits_stride}}, "logits") * w;
@@ -221,7 +267,6 @@ void launch_logits_adjust(const KuHipLogitsArgs& a, hipStream_t s) {
   d.history = (int32_t)a.history;
   d.bias_count = (int32_t)a.bias_count;
   d.mask_rows = (int32_t)a.mask_rows;
-  d.chunks = (uint32_t)((d.vocab + kChunk - 1) / kChunk);
   switch (a.dtype) {
     case KU_BF16: launch_t<GT_BF16, uint16_t>(d, a.out_dtype, (int64_t)a.rows, s); break;
     case KU_F16: launch_t<GT_F16, uint16_t>(d, a.out_dtype, (int64_t)a.rows, s); break;
