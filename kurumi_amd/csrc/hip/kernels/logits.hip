@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
     const int64_t m = a.mask_index ? a.mask_index[r] : r;
     if (m >= 0 && m < a.mask_rows) bits = reinterpret_cast<const uint8_t*>(a.mask + m * a.ms) + c0 / 8;
   }
+  const float inv = 1.f / rep;  // a second rounding, of 2^-24, in the place of a division for each logit
   uint32_t allowed[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -143,19 +144,27 @@ __global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
     const int i = (j * kThreads + tid) * V;
     if (i >= n) break;
     Vec<O, V> out;
+    float plain[V];
+    uint32_t biased = 0;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       float v = load_elem<DT, T, float>(in[j].e[e]);
-      const uint32_t c = counts ? count[i + e] : 0;
-      if (c) {
-        const uint32_t g = c & kCount;
-        if (c & ~kBiased) v = v > 0.f ? v / rep : v * rep;
-        if (g) v -= fmaf(freq, (float)g, pres);
-        if (c & kBiased) count[i + e] = __float_as_uint(v);  // for the bias, below
+      if (counts) {
+        // without a branch: of a wave's 64 places one is touched more often than not
+        const uint32_t c = count[i + e], g = c & kCount;
+        const float times = v > 0.f ? inv : rep, take = fmaf(freq, (float)g, pres);
+        v *= c & ~kBiased ? times : 1.f;
+        v -= g ? take : 0.f;
+        plain[e] = v;
+        biased |= c;
       }
       if (!(allowed[j] >> e & 1)) v = -INFINITY;
       out.e[e] = store_elem<OT, O>(v);
     }
+    if (biased & kBiased)  // for the bias, below
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (count[i + e] & kBiased) count[i + e] = __float_as_uint(plain[e]);
     if (i + V <= n) {
       *reinterpret_cast<Vec<O, V>*>(y + i) = out;
     } else {
