@@ -20,7 +20,6 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kLarge = 16, kSmall = 4;  // logits a thread: chunks of 8192 or 2048
-constexpr int kIds = 8;                 // vectors of four token ids a thread has in flight
 // A counter: how often the token was generated, and whether it is in the prompt and has biases.
 constexpr uint32_t kInPrompt = 0x80000000u, kBiased = 0x40000000u, kCount = kBiased - 1;
 
@@ -48,10 +47,10 @@ struct __attribute__((packed, aligned(sizeof(T)))) Vec {
 };
 
 template <int DT, class T, int OT, class O, int PER>
-__global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8))) logits_k(LogitsDev a) {
   // what the wider side moves 16 bytes at a time: consecutive lanes then write consecutive pieces
   constexpr int WIDE = 16 / (int)(sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O)), V = WIDE < PER ? WIDE : PER, N = PER / V;
-  constexpr int CHUNK = kThreads * PER;
+  constexpr int CHUNK = kThreads * PER, IDS = PER == kLarge ? 4 : 8;  // vectors of four token ids in flight
   __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
   __shared__ int repeats;
   const int64_t r = blockIdx.x / a.chunks, c0 = (int64_t)(blockIdx.x % a.chunks) * CHUNK;
@@ -107,10 +106,10 @@ __global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
     if (tid == 0) repeats = 0;
     __syncthreads();
     const int32_t* tok = a.tokens + r * a.ts;
-    for (int32_t i0 = 0; i0 < len; i0 += 4 * kIds * kThreads) {
-      Vec<int32_t, 4> id[kIds];
+    for (int32_t i0 = 0; i0 < len; i0 += 4 * IDS * kThreads) {
+      Vec<int32_t, 4> id[IDS];
 #pragma unroll
-      for (int j = 0; j < kIds; ++j) {
+      for (int j = 0; j < IDS; ++j) {
         const int32_t i = i0 + 4 * (j * kThreads + tid);
         if (i + 4 <= len) {
           id[j] = *reinterpret_cast<const Vec<int32_t, 4>*>(tok + i);
@@ -120,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) logits_k(LogitsDev a) {
         }
       }
 #pragma unroll
-      for (int j = 0; j < kIds; ++j) {
+      for (int j = 0; j < IDS; ++j) {
         const int32_t i = i0 + 4 * (j * kThreads + tid);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
