@@ -336,9 +336,7 @@ int32_t ku_hip_rope_freqs(size_t rot_dim, double base, uint32_t scaling, double 
  * whose row is outside [0, out_rows) is not stored (a padded batch: -1); rows that no token names
  * keep what they hold. Rows of one call have to differ: of two tokens with one row, either's values
  * may stay. An output may be its input itself (same pointer and strides; k and v then without
- * rows), otherwise they may not overlap. Any strides and alignments; where heads, strides and
- * pointers are multiples of 16 bytes (and rot_dim / 2 elements too), 16 bytes are moved at a time.
- * rot_dim is even, 0 to min(head_dim, 256). */
+X * rot_dim is even, 0 to min(head_dim, 256). */
 typedef struct KuHipRopeArgs {
   uint32_t size; /* sizeof(KuHipRopeArgs) */
   uint32_t dtype;

@@ -42,12 +42,12 @@ struct RopeDev {
 };
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // units a thread has in flight
 
 template <int N>
 struct Bits;
 template <> struct Bits<2> { using T = uint16_t; };
 template <> struct Bits<4> { using T = uint32_t; };
+template <> struct Bits<8> { using T = uint2; };
 template <> struct Bits<16> { using T = uint4; };
 
 // A unit is two vectors of V elements of one head: the low and the high features of V pairs (half
@@ -121,25 +121,22 @@ __global__ void __launch_bounds__(kThreads) rope_k(RopeDev a) {
     if (r.hi) *reinterpret_cast<W*>(r.y + r.hi) = r.x[1];
   };
 
-  Unit unit[kUnroll];
-  for (uint32_t base = threadIdx.x; base < total + threadIdx.x; base += kThreads * kUnroll) {
-#pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      unit[j].y = nullptr;
-      if (base + kThreads * j < total) unit[j] = load(base + kThreads * j);
-    }
-    if (base == threadIdx.x) {  // the first loads are on their way
-      for (uint32_t i = threadIdx.x; i < nt * half; i += kThreads) {
-        const uint32_t t = i / half;
-        const double turns = (double)a.positions[t0 + t] * a.turns[i - t * half];
-        float sn, cs;
-        sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
-        table[i] = make_float2(cs * a.scale, sn * a.scale);
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int j = 0; j < kUnroll; ++j) store(unit[j]);
+  uint32_t u = threadIdx.x;
+  Unit unit{};
+  if (u < total) unit = load(u);
+  // the first loads are on their way
+  for (uint32_t i = threadIdx.x; i < nt * half; i += kThreads) {
+    const uint32_t t = i / half;
+    const double turns = (double)a.positions[t0 + t] * a.turns[i - t * half];
+    float sn, cs;
+    sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+    table[i] = make_float2(cs * a.scale, sn * a.scale);
+  }
+  __syncthreads();
+  while (u < total) {
+    store(unit);
+    u += kThreads;
+    if (u < total) unit = load(u);
   }
 }
 
@@ -152,9 +149,10 @@ void launch_v(RopeDev& d, uint32_t q_heads, uint32_t k_heads, uint32_t v_heads, 
   d.q_units = q_heads * (d.turned + d.copied);
   d.qk_units = d.q_units + k_heads * (d.turned + d.copied);
   d.units = d.qk_units + v_heads * d.v_units;
-  // Work-groups of about 8 units a thread (two rounds of loads) where that leaves enough of them, of
-  // one where it does not: a few tokens are spread over their heads.
-  const int64_t all = d.tokens * (int64_t)d.units, want = all / (8 * kThreads) >= 4 * (int64_t)cu_count() ? 8 * kThreads : kThreads;
+  // Work-groups of about two units a thread where that leaves enough of them (8192 tokens of 48 heads of
+  // 128, bf16: 41.8 us; 47 with eight a thread, 56 with four of those in flight), of one where it does not:
+  // a few tokens are spread over their heads.
+  const int64_t all = d.tokens * (int64_t)d.units, want = all / (2 * kThreads) >= 4 * (int64_t)cu_count() ? 2 * kThreads : kThreads;
   d.block_tokens = (uint32_t)std::max<int64_t>(1, std::min<int64_t>({want / d.units, d.tokens, 64}));
   d.block_units = d.block_tokens > 1 ? d.units : (uint32_t)std::min<int64_t>(d.units, std::max<int64_t>(want, (d.units + 65534) / 65535));
   const dim3 grid((unsigned)((d.tokens + d.block_tokens - 1) / d.block_tokens), (d.units + d.block_units - 1) / d.block_units);
@@ -251,18 +249,25 @@ void launch_rope(const KuHipRopeArgs& a, hipStream_t s) {
   for (uint32_t i = 0; i < d.rot / 2; ++i) d.turns[i] = (a.inverse ? -a.freqs[i] : a.freqs[i]) / 6.283185307179586476925;
   const uint32_t qh = a.q ? (uint32_t)a.q_heads : 0, kh = a.k ? (uint32_t)a.kv_heads : 0, vh = a.v ? (uint32_t)a.kv_heads : 0;
   const bool half = a.layout == KU_ROPE_HALF;
-  // 16 bytes at a time where everything is made of them
-  const int64_t v = a.dtype == KU_F32 ? 4 : 8;
-  bool wide = d.dim % v == 0 && (d.rot / 2) % v == 0;
-  for (const RopeSide* x : {&d.q, &d.k, &d.v})
-    if (x->in)
-      wide = wide && aligned_to(x->in, 16) && aligned_to(x->out, 16) && x->in_token % v == 0 && x->in_head % v == 0 &&
+  // as many bytes at a time, up to 16, as everything is made of
+  auto made_of = [&](int64_t v) {
+    bool ok = d.dim % v == 0 && (d.rot / 2) % v == 0;
+    const size_t bytes = (size_t)v * (a.dtype == KU_F32 ? 4 : 2);
+    for (const RopeSide* x : {&d.q, &d.k, &d.v})
+      if (x->in)
+        ok = ok && aligned_to(x->in, bytes) && aligned_to(x->out, bytes) && x->in_token % v == 0 && x->in_head % v == 0 &&
              x->out_row % v == 0 && x->out_head % v == 0;
+    return ok;
+  };
   auto go = [&](auto dt, auto elem) {
     constexpr int DT = decltype(dt)::value;
     using T = decltype(elem);
-    if (wide)
-      launch_v<DT, T, 16 / (int)sizeof(T)>(d, qh, kh, vh, half, s);
+    if (sizeof(T) == 2 && made_of(8))
+      launch_v<DT, T, sizeof(T) == 2 ? 8 : 4>(d, qh, kh, vh, half, s);
+    else if (made_of(4))
+      launch_v<DT, T, 4>(d, qh, kh, vh, half, s);
+    else if (made_of(2))
+      launch_v<DT, T, 2>(d, qh, kh, vh, half, s);
     else
       launch_v<DT, T, 1>(d, qh, kh, vh, half, s);
   };
