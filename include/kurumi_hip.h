@@ -336,7 +336,9 @@ int32_t ku_hip_rope_freqs(size_t rot_dim, double base, uint32_t scaling, double 
  * whose row is outside [0, out_rows) is not stored (a padded batch: -1); rows that no token names
  * keep what they hold. Rows of one call have to differ: of two tokens with one row, either's values
  * may stay. An output may be its input itself (same pointer and strides; k and v then without
-X * rot_dim is even, 0 to min(head_dim, 256). */
+ * rows), otherwise they may not overlap. Any strides and alignments; as many bytes are moved at a time,
+ * up to 16, as heads, rot_dim / 2, strides and pointers are made of.
+ * rot_dim is even, 0 to min(head_dim, 256). */
 typedef struct KuHipRopeArgs {
   uint32_t size; /* sizeof(KuHipRopeArgs) */
   uint32_t dtype;
