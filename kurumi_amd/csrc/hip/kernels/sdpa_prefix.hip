@@ -780,42 +780,45 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     run_unit<DT, D, false>(g, second, unit, lds, sh);
 }
 
-// Joins the partial results of a row, one wave a row: the slots' weights in the lanes, then eight slots'
-// outputs at a time.
-template <int DT, int D>
+// Joins the partial results of rows, eight slots a lane at a time: with SIDE slots of a row side by side
+// in a wave, or several rows beside each other. One round of loads where that covers the slots.
+template <int DT, int D, int SIDE>
 __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
+  constexpr int L = D / 4, ROWS = 64 / (L * SIDE), U = 8;  // lanes a slot's output takes, rows of a wave
   __shared__ float lds[4][kSdpaMaxDim];
   const SdpaDev& a = g.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-  if (row >= (int64_t)a.batch * a.q_len * a.q_heads) return;
-  const int n = g.p.slots;
-  const float2* ml = g.ml + row * n;
-  constexpr int L = D / 4, S = 64 / L;  // lanes a slot's output takes, slots side by side
-  const int ch = lane % L, sub = lane / L;
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, ml[i].x);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  const float from = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ch = lane % L, sub = lane / L % SIDE;
+  const int rows = a.batch * a.q_len * a.q_heads, row0 = ((int)blockIdx.x * 4 + wave) * ROWS, row = row0 + lane / (L * SIDE);
+  const bool there = row < rows;
+  const int n = there ? g.p.slots : 0;
+  const float2* ml = g.ml + (int64_t)row * g.p.slots;
+  const f32x4* po = reinterpret_cast<const f32x4*>(g.po + (int64_t)row * g.p.slots * D) + ch;
+  float m = -INFINITY, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const f32x4* po = reinterpret_cast<const f32x4*>(g.po + row * n * D) + ch;
-  for (int i0 = 0; i0 < n; i0 += 8 * S) {
-    f32x4 x[8];
-    float2 y[8];
+  for (int i0 = 0; i0 < g.p.slots; i0 += U * SIDE) {
+    f32x4 x[U];
+    float2 y[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = i0 + j * S + sub;
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + j * SIDE + sub;
       x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
       y[j] = make_float2(-INFINITY, 0.f);
       if (i < n) {
-        x[j] = po[(int64_t)i * L];
+        x[j] = po[i * L];
         y[j] = ml[i];
       }
     }
+    float top = m;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < U; ++j) top = fmaxf(top, y[j].x);
+#pragma unroll
+    for (int o = L; o < L * SIDE; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float from = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - from);
+    m = top;
+    l *= old;
+    acc *= old;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
       const float w = __builtin_amdgcn_exp2f(y[j].x - from);  // 0 for a slot that saw nothing
       l = fmaf(w, y[j].y, l);
       acc += x[j] * w;
@@ -823,18 +826,26 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
   }
   // the slots side by side are added in one order in every lane
 #pragma unroll
-  for (int o = L; o < 64; o <<= 1) {
+  for (int o = L; o < L * SIDE; o <<= 1) {
     l += __shfl_xor(l, o, 64);
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] += __shfl_xor(acc[k], o, 64);
   }
-  const RowAt at(g.p, (int)row);
-  if (__builtin_amdgcn_ballot_w64(bad_sum(l) || bad_sum(acc[0]) || bad_sum(acc[1]) || bad_sum(acc[2]) || bad_sum(acc[3])) != 0 || l == 0.f) {
-    sdpa_one<DT>(a, at.b, at.t, at.h, lds[wave]);
-    return;
+  const RowAt at(g.p, there ? row : 0);
+  // a row's lanes that are not finite: the whole row is done again
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(
+      there && (l == 0.f || bad_sum(l) || bad_sum(acc[0]) || bad_sum(acc[1]) || bad_sum(acc[2]) || bad_sum(acc[3])));
+  constexpr uint64_t LANES = L * SIDE == 64 ? ~0ull : (1ull << (L * SIDE % 64)) - 1;
+  if (there && (bad >> (lane / (L * SIDE) * (L * SIDE)) & LANES) == 0) {
+    if (sub == 0) write_out<DT>(a, at, ch * 4, acc * (1.f / l));
+    if (a.lse && ch == 0 && sub == 0) a.lse[row] = (m + __builtin_amdgcn_logf(l)) * LN2;
   }
-  if (sub == 0) write_out<DT>(a, at, ch * 4, acc * (1.f / l));
-  if (a.lse && lane == 0) a.lse[row] = (m + __builtin_amdgcn_logf(l)) * LN2;
+  if (bad)
+    for (int i = 0; i < ROWS; ++i)
+      if (bad >> (i * L * SIDE) & LANES) {
+        const RowAt again(g.p, row0 + i);
+        sdpa_one<DT>(a, again.b, again.t, again.h, lds[wave]);
+      }
 }
 
 SdpaDev device_args(const KuHipSdpaPrefixArgs& a) {
@@ -921,7 +932,13 @@ void launch_d(const SdpaArgs& g, hipStream_t s) {
   const unsigned groups = 8 * (unsigned)((g.p.part[0].units + 7) / 8 + (g.p.part[1].units + 7) / 8);
   if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D>), dim3(groups), dim3(256), 0, s, g);
   const int64_t rows = (int64_t)g.a.batch * g.a.q_len * g.a.q_heads;
-  if (g.p.slots != 1) hipLaunchKernelGGL((sdpa_join_k<DT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, g);
+  if (g.p.slots == 1) return;
+  // few slots: several rows a wave (32768 rows of 64, two slots: 14 us with a wave a row)
+  constexpr int S = 256 / D;
+  if (g.p.slots <= 8)
+    hipLaunchKernelGGL((sdpa_join_k<DT, D, 1>), dim3((unsigned)((rows + 4 * S - 1) / (4 * S))), dim3(256), 0, s, g);
+  else
+    hipLaunchKernelGGL((sdpa_join_k<DT, D, S>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, g);
 }
 template <int DT>
 void launch_t(const SdpaArgs& g, int d, hipStream_t s) {
