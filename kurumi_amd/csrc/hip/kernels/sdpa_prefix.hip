@@ -117,14 +117,16 @@ __device__ __forceinline__ float other_half(float x) {
   return __uint_as_float((threadIdx.x & 32) ? sw[0] : sw[1]);
 }
 
-template <int DT, int D>
+// Rows of keys lie in LDS as D features, of which the products take the first DR (heads of 65 to 96
+// features as 96 of 128: a quarter of the products less).
+template <int DT, int D, int DR>
 struct Tile {
   static constexpr int ES = DT == GT_F32 ? 4 : 2;
   static constexpr int RB = D * ES;          // bytes of a row in LDS
   static constexpr int CPR = RB / 16;        // 16-byte chunks of a row
   static constexpr int KT = 32 * RB;         // bytes of 32 keys
-  static constexpr int DS = CPR / 2;         // chunk pairs: steps of S^T
-  static constexpr int DTL = D / 32;         // 32-row tiles of O^T
+  static constexpr int DS = DR * ES / 32;    // chunk pairs: steps of S^T
+  static constexpr int DTL = DR / 32;        // 32-row tiles of O^T
   static constexpr int SB = DT == GT_F32 ? 1 : 2;  // 32-key tiles of a shared block
   // shared: K and V, two buffers each; solo: K and V of every wave
   static constexpr int LDS = std::max(4 * SB * KT, 4 * 2 * KT);
@@ -141,9 +143,9 @@ struct Tile {
 };
 
 // One wave's 32 rows of a tile: Q fragments, running maximum, sum and O.
-template <int DT, int D>
+template <int DT, int D, int DR>
 struct Rows {
-  using T = Tile<DT, D>;
+  using T = Tile<DT, D, DR>;
   u32x4 q[T::DS];
   f32x16 o[T::DTL];
   float m, l;  // m in powers of two, already times scale
@@ -276,9 +278,9 @@ struct Rows {
 };
 
 // A run of keys of one kv head, prefix or own, and the DMA of tiles of it.
-template <int DT, int D>
+template <int DT, int D, int DR>
 struct Keys {
-  using T = Tile<DT, D>;
+  using T = Tile<DT, D, DR>;
   static constexpr int RPD = 1024 / T::RB;  // rows of one DMA instruction
   const char *k, *v;     // row 0 of the head
   int64_t stride;        // bytes a row
@@ -361,10 +363,10 @@ struct Keys {
 };
 
 // the prefix, or sequence b's own `n` keys
-template <int DT, int D>
-__device__ __forceinline__ Keys<DT, D> keys_of(const SdpaDev& a, bool own, int b, int n, int kvh) {
+template <int DT, int D, int DR>
+__device__ __forceinline__ Keys<DT, D, DR> keys_of(const SdpaDev& a, bool own, int b, int n, int kvh) {
   using E = typename SdpaElem<DT>::T;
-  Keys<DT, D> S;
+  Keys<DT, D, DR> S;
   const bool paged = own && a.page_shift >= 0;
   const int64_t base = kvh * (own ? a.head : a.phead) + (own && !paged ? b * a.seq_rows * a.row : 0);
   S.k = reinterpret_cast<const char*>(static_cast<const E*>(own ? a.k : a.pk) + base);
@@ -461,9 +463,9 @@ struct SdpaShared {
 
 // One unit: a tile of rows against a split of its keys. SHARED: four waves of 32 rows share blocks of
 // keys; else the waves deal the blocks of one tile of 32 rows among them.
-template <int DT, int D, bool SHARED>
+template <int DT, int D, int DR, bool SHARED>
 __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id, unsigned char* lds_raw, SdpaShared& sh) {
-  using T = Tile<DT, D>;
+  using T = Tile<DT, D, DR>;
   using E = typename SdpaElem<DT>::T;
   constexpr int ROWS = SHARED ? 128 : 32;
   KU_LDS unsigned char* lds = (KU_LDS unsigned char*)lds_raw;
@@ -493,7 +495,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   int split_first, split_last;
   split_range(part.by_splits, np + no, split, split_first, split_last);
   bool none = false;
-  Rows<DT, D> R;
+  Rows<DT, D, DR> R;
   R.clear();
   R.limit = 0;
   if (threadIdx.x == 0) sh.redo = sh.none = 0;
@@ -513,11 +515,11 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   for (int seg = second; seg <= (int)(second || joint); ++seg) {
     const int first = seg ? std::max(split_first, np) - np : split_first, last = seg ? split_last - np : std::min(split_last, np);
     if (first >= last) continue;
-    Keys<DT, D> S = keys_of<DT, D>(a, seg, b, own_len, kvh);
+    Keys<DT, D, DR> S = keys_of<DT, D, DR>(a, seg, b, own_len, kvh);
     const int all = seg ? 0 : a.prefix;  // keys that every query sees
     if constexpr (SHARED) {
       // Four waves of 32 rows over blocks of BK keys, two buffers for K and two for V.
-      constexpr int BK = 32 * T::SB, TB = T::SB * T::KT, N = BK / Keys<DT, D>::RPD / 4;
+      constexpr int BK = 32 * T::SB, TB = T::SB * T::KT, N = BK / Keys<DT, D, DR>::RPD / 4;
       const bool active = row0 < nrows;  // a wave past the last row only fetches
       auto kbuf = [&](int i) { return lds + i * TB; };
       auto vbuf = [&](int i) { return lds + (2 + i) * TB; };
@@ -560,8 +562,8 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
         // block blk's softmax, are issued between its exponentials, each fragment of K read two products
         // ahead (a scheduling barrier after each group keeps them so). Two blocks a trip, so that the
         // parity of the buffers is a constant.
-        constexpr int NM = 2 * T::DS, PPM = 16 / NM;
-        static_assert(T::SB == 2 && NM * PPM == 16, "exponential pairs a product");
+        constexpr int NM = 2 * T::DS;  // products of a block's scores, among 16 exponential pairs
+        static_assert(T::SB == 2 && NM <= 16);
         auto step = [&](int blk, f32x16 (&sc)[2], f32x16 (&sn)[2], auto par) __attribute__((always_inline)) {
           constexpr int PAR = decltype(par)::value;
           if (blk + 2 < last) fetch(blk + 2, IsK, kbuf(PAR));
@@ -585,8 +587,8 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
             for (int m = 0; m < NM; ++m) {
               if (m + 2 < NM) kf[(m + 2) % 3] = kread(m + 2);
 #pragma unroll
-              for (int e = 0; e < PPM; ++e) {
-                const int i = m * PPM + e, te = i >> 3, v2 = i & 7;
+              for (int i = 16 * m / NM; i < 16 * (m + 1) / NM; ++i) {
+                const int te = i >> 3, v2 = i & 7;
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2], c, em));
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2 + 1], c, em));
                 const uint32_t pp = pack2<DT>(p0, p1);
@@ -621,7 +623,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
     } else {
       // The waves take blocks of 32 keys in turn, each by itself: K of its next block is fetched once this
       // one's scores are done, V once its products are, so either is on its way while the other is used.
-      constexpr int N = 32 / Keys<DT, D>::RPD;
+      constexpr int N = 32 / Keys<DT, D, DR>::RPD;
       KU_LDS unsigned char *K = lds + wave * 2 * T::KT, *V = K + T::KT;
       int64_t off[N];
       auto fetch_k = [&](int blk) {
@@ -734,8 +736,8 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
     if (wave == 0 && h == 0) sh.ml[0][lane] = make_float2(m, l);
     __syncthreads();
     const int rows = std::min(32, nrows - row0);
-    for (int i = threadIdx.x; i < rows * CH; i += 256) {
-      const int r = i / CH, ch = i % CH;
+    for (int i = threadIdx.x; i < rows * (DR / 4); i += 256) {
+      const int r = i / (DR / 4), ch = i % (DR / 4);
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) o += *(const KU_LDS f32x4*)(lds + w * 32 * D * 4 + r * D * 4 + ((ch ^ (r & (CH - 1) & 31)) << 4));
@@ -766,18 +768,18 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   }
 }
 
-template <int DT, int D>
+template <int DT, int D, int DR>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) sdpa_tiles_k(SdpaArgs g) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[Tile<DT, D>::LDS];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[Tile<DT, D, DR>::LDS];
   __shared__ SdpaShared sh;
   touch_arguments<SdpaArgs>();
   bool second;
   int unit;
   if (!unit_of(g.p, blockIdx.x, second, unit)) return;
   if (g.p.part[second].shared)
-    run_unit<DT, D, true>(g, second, unit, lds, sh);
+    run_unit<DT, D, DR, true>(g, second, unit, lds, sh);
   else
-    run_unit<DT, D, false>(g, second, unit, lds, sh);
+    run_unit<DT, D, DR, false>(g, second, unit, lds, sh);
 }
 
 // Joins the partial results of rows, eight slots a lane at a time: with SIDE slots of a row side by side
@@ -804,7 +806,7 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
       x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
       y[j] = make_float2(-INFINITY, 0.f);
       if (i < n) {
-        x[j] = po[i * L];
+        if (ch * 4 < a.dim) x[j] = po[i * L];
         y[j] = ml[i];
       }
     }
@@ -927,10 +929,10 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
 
 int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
-template <int DT, int D>
+template <int DT, int D, int DR>
 void launch_d(const SdpaArgs& g, hipStream_t s) {
   const unsigned groups = 8 * (unsigned)((g.p.part[0].units + 7) / 8 + (g.p.part[1].units + 7) / 8);
-  if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D>), dim3(groups), dim3(256), 0, s, g);
+  if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR>), dim3(groups), dim3(256), 0, s, g);
   const int64_t rows = (int64_t)g.a.batch * g.a.q_len * g.a.q_heads;
   if (g.p.slots == 1) return;
   // few slots: several rows a wave (32768 rows of 64, two slots: 14 us with a wave a row)
@@ -943,9 +945,9 @@ void launch_d(const SdpaArgs& g, hipStream_t s) {
 template <int DT>
 void launch_t(const SdpaArgs& g, int d, hipStream_t s) {
   switch (d) {
-    case 32: launch_d<DT, 32>(g, s); break;
-    case 64: launch_d<DT, 64>(g, s); break;
-    default: launch_d<DT, 128>(g, s); break;
+    case 32: launch_d<DT, 32, 32>(g, s); break;
+    case 64: launch_d<DT, 64, 64>(g, s); break;
+    default: g.a.dim <= 96 ? launch_d<DT, 128, 96>(g, s) : launch_d<DT, 128, 128>(g, s); break;
   }
 }
 
