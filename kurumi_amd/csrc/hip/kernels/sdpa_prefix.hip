@@ -81,7 +81,8 @@ struct SdpaPlan {
     int units = 0;               // work-groups: tiles times splits of all of them
     Div by_tiles, by_splits;
   } part[2];
-  int slots = 0;  // partial results a row
+  int slots = 0;        // partial results a row
+  bool sorted = false;  // the own keys' units by their sequences' lengths
   Div by_kv, by_group, by_seq, by_q_len, by_heads;  // kv heads; q heads of one; a sequence's rows; its queries; q heads
 };
 
@@ -414,6 +415,20 @@ __device__ __forceinline__ bool unit_of(const SdpaPlan& p, int i, bool& second, 
   return true;
 }
 
+// The sequence of a batch of up to 64 that unit position i of the own keys takes: the longest first, so that
+// the last work-groups to start are the shortest (64 sequences of 16 to 1024 keys beside 8192 shared ones:
+// see the table), and by turns over the XCDs, each of which has a run of positions.
+__device__ __forceinline__ int longest_first(const SdpaDev& a, int i) {
+  const int lane = threadIdx.x & 63, n = a.batch;
+  const int g = n & 7 ? (n & 3 ? (n & 1 ? 1 : 2) : 4) : 8, period = n / g;
+  const int want = i * 8 % n + i / period;
+  // ties by number: lengths and lanes in one key
+  const int key = lane < n ? (sdpa_len(a, lane) << 6 | (63 - lane)) : -1;
+  int rank = 0;
+  for (int j = 0; j < n; ++j) rank += __builtin_amdgcn_readlane(key, j) > key;
+  return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < n && rank == want));
+}
+
 // where a query's row lies
 struct RowAt {
   int b, t, h;
@@ -479,7 +494,8 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   int tile, kvh, split;
   id = part.by_tiles.split(id, tile);
   id = g.p.by_kv.split(id, kvh);  // heads before splits: their rows lie next to each other
-  const int b = part.by_splits.split(id, split);
+  int b = part.by_splits.split(id, split);
+  if (second && g.p.sorted) b = longest_first(a, b);
   const int per_seq = a.q_len * a.group, nrows = pooled ? a.batch * per_seq : per_seq;
   const int row0 = tile * ROWS + (SHARED ? wave * 32 : 0);  // of this wave
   const int own_len = pooled ? 0 : __builtin_amdgcn_readfirstlane(sdpa_len(a, b));
@@ -919,6 +935,8 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max, 2 * cu);
   }
   p.slots = p.part[0].splits + p.part[1].splits;
+  // keys fit 25 bits beside a lane's number; one round of work-groups needs no order
+  p.sorted = a.batch > 1 && a.batch <= 64 && a.own_max < (1u << 25) && p.part[1].units > cu;
   p.by_kv = Div(kv);
   p.by_group = Div(group);
   p.by_seq = Div(per_seq);
