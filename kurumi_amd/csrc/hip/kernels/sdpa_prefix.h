@@ -50,9 +50,10 @@ struct SdpaElem<GT_F32> {
   static constexpr int V = 4;
 };
 
-// One query by one wave, from the definition: the maximum over the keys it sees, then the sums. Only
-// keys that it sees are read, and infinities and NaN come out as the definition has them: the tiled
-// kernels leave queries to it whose sums are not finite. `lds`: kSdpaMaxDim floats of the wave.
+// One query by one wave, from the definition: the maximum over the keys it sees, the sum of their
+// probabilities, then the values by probabilities that add up to one, so that nothing overflows that the
+// result does not. Only keys that it sees are read, and infinities and NaN come out as the definition has
+// them: the tiled kernels leave queries to it whose sums are not finite. `lds`: kSdpaMaxDim floats of the wave.
 template <int DT>
 __device__ void sdpa_one(const SdpaDev& a, int b, int t, int h, float* lds) {
   using T = typename SdpaElem<DT>::T;
@@ -100,10 +101,16 @@ __device__ void sdpa_one(const SdpaDev& a, int b, int t, int h, float* lds) {
   any = __builtin_amdgcn_ballot_w64(any) != 0;
   nan = __builtin_amdgcn_ballot_w64(nan) != 0;
   float l = 0.f, acc[kSdpaMaxDim / 64] = {};
+  for (int64_t j = lane; j < n; j += 64) {
+    const int64_t off = offset(j);
+    if (off >= 0) l += expf(score(j, off) - m);
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o, 64);
+  const float inv = 1.f / l;
   for (int64_t j0 = 0; j0 < n; j0 += 64) {
     const int64_t j = j0 + lane, off = j < n ? offset(j) : -1;
-    const float p = off < 0 ? 0.f : expf(score(j, off) - m);
-    l += p;
+    const float p = off < 0 ? 0.f : expf(score(j, off) - m) * inv;
     const int left = n - j0 < 64 ? (int)(n - j0) : 64;
     for (int i = 0; i < left; ++i) {
       const int64_t oi = ((int64_t)__builtin_amdgcn_readlane((int)(off >> 32), i) << 32) |
@@ -116,12 +123,10 @@ __device__ void sdpa_one(const SdpaDev& a, int b, int t, int h, float* lds) {
         if (lane + 64 * c < a.dim) acc[c] = fmaf(pi, load_elem<DT, T, float>(val[lane + 64 * c]), acc[c]);
     }
   }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o, 64);
   T* out = static_cast<T*>(a.o) + b * a.ob + t * a.ot + h * a.oh;
 #pragma unroll
   for (int c = 0; c < kSdpaMaxDim / 64; ++c)
-    if (lane + 64 * c < a.dim) out[lane + 64 * c] = store_elem<DT, T, float>(any ? acc[c] / l : 0.f);
+    if (lane + 64 * c < a.dim) out[lane + 64 * c] = store_elem<DT, T, float>(any ? acc[c] : 0.f);
   if (a.lse && lane == 0)
     a.lse[((int64_t)b * a.q_len + t) * a.q_heads + h] = nan ? NAN : isinf(m) ? m : m + logf(l);
 }

@@ -377,7 +377,7 @@ __device__ __forceinline__ Keys<DT, D, DR> keys_of(const SdpaDev& a, bool own, i
   S.table = paged ? a.pages + b * a.per_seq : nullptr;
   S.shift = paged ? a.page_shift : 0;
   S.npages = a.npages;
-  S.flat = !paged && S.stride > 0 && S.stride < (1 << 25);
+  S.flat = !paged && S.stride >= a.dim * (int)sizeof(E) && S.stride < (1 << 25);  // rows apart, 64 of them within 2 GiB
   return S;
 }
 
@@ -981,8 +981,8 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
   require(a.q_heads % a.kv_heads == 0, "q_heads must be a multiple of kv_heads");
   const size_t most = 0x7fffffff;
   require(a.batch <= most && a.q_len <= most && a.q_heads <= most &&
-              (__int128)a.batch * a.q_len * a.q_heads <= (__int128)most,
-          "more than 2^31 - 1 queries");
+              (__int128)a.batch * a.q_len * a.q_heads <= (__int128)1 << 30,
+          "more than 2^30 queries");
   require(a.prefix_len <= most - 256 && a.own_max <= most - 256 && a.q_len <= most - 256, "more than 2^31 - 257 keys");
   auto strides16 = [&](std::initializer_list<int64_t> s) {
     for (int64_t x : s) require(x % v == 0, "strides must be multiples of 16 bytes");

@@ -153,7 +153,7 @@ def test_sdpa_prefix_accepts(kw):
     (dict(size=8), "sizeof"), (dict(dtype=int(DType.F8E4M3)), "dtype"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
     (dict(scale=math.nan), "scale"), (dict(head_dim=0), "head_dim"), (dict(head_dim=60), "head_dim"), (dict(head_dim=136), "head_dim"),
     (dict(q_len=0), "positive"), (dict(kv_heads=0), "positive"), (dict(kv_heads=3), "multiple of kv_heads"), (dict(batch=1 << 31), "queries"),
-    (dict(prefix_len=1 << 31), "keys"), (dict(own_max=1 << 31), "keys"), (dict(q_len=1 << 30, batch=1), "queries"),
+    (dict(prefix_len=1 << 31), "keys"), (dict(own_max=1 << 31), "keys"), (dict(q_len=1 << 28, batch=1), "queries"),
     (dict(q=None), "null device pointer"), (dict(out=None), "null device pointer"), (dict(prefix_v=None), "null device pointer"),
     (dict(own_k=None), "null device pointer"), (dict(own_lens=None), "own_lens"), (dict(q=P + 8), "16-byte aligned"),
     (dict(lse=3 * P + 2), "4-byte aligned"), (dict(scratch=P + 4), "scratch must be 16-byte"), (dict(q_head_stride=60), "16 bytes"),

@@ -111,6 +111,16 @@ SIZES = [  # batch, q_len, q_heads, kv_heads, d, prefix, own_max, page
     (2, 150, 6, 2, 128, 70, 170, 32),
     (1, 300, 2, 2, 40, 100, 300, 0),
     (7, 17, 3, 3, 128, 0, 50, 16),
+    (2, 1, 64, 1, 64, 500, 33, 0),        # many heads on one kv head: a whole tile of one sequence's rows
+    (2, 1, 4, 2, 64, 0, 700, 8),          # more pages than a wave has lanes
+    (1, 1, 2, 1, 32, 3, 300, 1),          # a page for each key
+    (1, 140, 2, 1, 64, 50, 400, 1),
+    (64, 1, 8, 8, 64, 100, 130, 16),      # more units than CUs: the longest sequences first
+    (61, 1, 8, 8, 32, 64, 40, 0),
+    (70, 1, 8, 4, 64, 31, 129, 32),       # more sequences than a wave has lanes
+    (20, 1, 16, 4, 128, 5000, 600, 16),   # many splits of either part
+    (40, 3, 8, 2, 128, 1500, 20, 0),      # shared tiles over the prefix
+    (3, 257, 4, 2, 96, 700, 300, 0),      # joint tiles, split
 ]
 
 
@@ -190,6 +200,37 @@ def test_large_scores(hip, dt):
 def test_strides(hip, dt, heads_first, pad):
     print(f"sdpa_prefix strides {dt.name} {heads_first} {pad}", flush=True)
     Case(dt, 3, 2, 6, 3, 72, 150, 70, heads_first=heads_first, pad=pad).check(hip)
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("nb,nt", [(2, 1), (40, 2), (2, 70)])
+def test_rows_of_keys_that_repeat_or_overlap(hip, dt, nb, nt):
+    """A row stride of nothing, and one of less than a row: the keys are views of each other."""
+    print(f"sdpa_prefix overlapping rows {dt.name} {nb} {nt}", flush=True)
+    d, prefix = 64, 90
+    c = Case(dt, nb, nt, 2, 1, d, prefix, 0)
+    for stride in (0, 16):
+        flat = narrow(np.random.default_rng(5).standard_normal(prefix * stride + d), dt)
+        c.pk = c.pv = np.stack([flat[j * stride : j * stride + d] for j in range(prefix)])[:, None]
+        buf = dev(flat)
+        hip.sdpa_prefix(c.args(prefix_k=buf.ptr, prefix_v=buf.ptr, prefix_row_stride=stride, prefix_head_stride=0))
+        o, l = c.results()
+        wo, wl, to, tl = c.want()
+        assert_within(widen(o, dt), wo, to, f"out, stride {stride}")
+        assert_within(l, wl, tl, f"lse, stride {stride}")
+
+
+@pytest.mark.parametrize("dt", [DType.F32, DType.BF16])
+def test_values_near_the_largest(hip, dt):
+    """Sums of values that overflow where their mean does not."""
+    for nb, nt in ((2, 1), (40, 2), (1, 130)):
+        c = Case(dt, nb, nt, 2, 1, 32, 70, 10, lens=[10] * nb)
+        big = narrow(np.array([2.5e38], np.float32), dt)[0]
+        c.pv[:, 0, 3], c.v[:, 0, 3] = big, big
+        o, _ = c.run(hip)
+        want = float(widen(np.array([big]), dt)[0])
+        # the probabilities add up to one within the sums' and the output's roundings
+        assert (np.abs(widen(o[..., 3], dt) / want - 1) < (100 * 2.0 ** -24 if dt == DType.F32 else 2.0 ** -8)).all()
 
 
 def test_strides_of_queries_and_outputs(hip):
