@@ -95,6 +95,13 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8
     allowed[j] = bits && i < n ? bits[i / 8] >> (i & 7) : 0xffu;
   }
   const bool counts = len > 0 || e1 > e0;
+  // a thread's first bias, loaded beside the tokens
+  int32_t bias_id = -1;
+  float bias_value = 0.f;
+  if (e0 + tid < e1) {
+    bias_id = a.bias_ids[e0 + tid];
+    bias_value = a.bias_values[e0 + tid];
+  }
   // the place of token v in the chunk, or one past it
   auto place = [&](int32_t v) {
     const uint64_t at = (uint64_t)((int64_t)v - c0);
@@ -133,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8
       }
     }
     for (int32_t e = e0 + tid; e < e1; e += kThreads) {
-      const int at = place(a.bias_ids[e]);
+      const int at = place(e == e0 + tid ? bias_id : a.bias_ids[e]);
       if (at != CHUNK && (atomicOr(&count[at], kBiased) & kBiased)) repeats = 1;
     }
     __syncthreads();
@@ -185,10 +192,10 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8
     __syncthreads();
   }
   for (int32_t e = e0 + tid; e < e1; e += kThreads) {
-    const int at = place(a.bias_ids[e]);
+    const int at = place(e == e0 + tid ? bias_id : a.bias_ids[e]);
     if (at == CHUNK || (bits && !(bits[at / 8] >> (at & 7) & 1))) continue;
     const float v = __uint_as_float(count[at]);
-    y[at] = store_elem<OT, O>(again ? v : v + a.bias_values[e]);
+    y[at] = store_elem<OT, O>(again ? v : v + (e == e0 + tid ? bias_value : a.bias_values[e]));
   }
 }
 
