@@ -293,6 +293,12 @@ struct Keys {
   int page = 0;          // the blocks then loads nothing that the compiler would wait for
   bool none = false;     // a page that is none was met
 
+  // The pages of the keys from j0 on, one a lane.
+  __device__ __forceinline__ void hold(int j0) {
+    const int last = (n - 1) >> shift;
+    held = j0 >> shift;
+    page = table[held + (threadIdx.x & 63) < last ? held + (threadIdx.x & 63) : last];
+  }
   // Byte offsets of the rows that this wave's share (of WAVES) of KEYS keys from j0 on reads.
   template <int KEYS, int WAVES>
   __device__ __forceinline__ void rows(int j0, int wave, int64_t (&off)[KEYS / RPD / WAVES]) {
@@ -301,12 +307,8 @@ struct Keys {
     if (flat) return;
     const int lane = threadIdx.x & 63, r = lane / T::CPR;
     if (table) {
-      const int p0 = j0 >> shift, p1 = (j0 + KEYS - 1 < n ? j0 + KEYS - 1 : n - 1) >> shift;
-      if (held < 0 || p1 >= held + 64) {
-        held = p0;
-        const int last = (n - 1) >> shift;
-        page = table[p0 + lane < last ? p0 + lane : last];
-      }
+      const int p1 = (j0 + KEYS - 1 < n ? j0 + KEYS - 1 : n - 1) >> shift;
+      if (held < 0 || p1 >= held + 64) hold(j0);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         int j = j0 + (i * WAVES + wave) * RPD + r;
@@ -418,15 +420,18 @@ __device__ __forceinline__ bool unit_of(const SdpaPlan& p, int i, bool& second, 
 // The sequence of a batch of up to 64 that unit position i of the own keys takes: the longest first, so that
 // the last work-groups to start are the shortest (64 sequences of 16 to 1024 keys beside 8192 shared ones:
 // see the table), and by turns over the XCDs, each of which has a run of positions.
-__device__ __forceinline__ int longest_first(const SdpaDev& a, int i) {
+__device__ __forceinline__ int longest_first(const SdpaDev& a, int i, int& len) {
   const int lane = threadIdx.x & 63, n = a.batch;
   const int g = n & 7 ? (n & 3 ? (n & 1 ? 1 : 2) : 4) : 8, period = n / g;
   const int want = i * 8 % n + i / period;
   // ties by number: lengths and lanes in one key
   const int key = lane < n ? (sdpa_len(a, lane) << 6 | (63 - lane)) : -1;
   int rank = 0;
-  for (int j = 0; j < n; ++j) rank += __builtin_amdgcn_readlane(key, j) > key;
-  return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < n && rank == want));
+#pragma unroll
+  for (int j = 0; j < 64; ++j) rank += __builtin_amdgcn_readlane(key, j) > key;
+  const int b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < n && rank == want));
+  len = __builtin_amdgcn_readlane(key, b) >> 6;
+  return b;
 }
 
 // where a query's row lies
@@ -495,10 +500,13 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   id = part.by_tiles.split(id, tile);
   id = g.p.by_kv.split(id, kvh);  // heads before splits: their rows lie next to each other
   int b = part.by_splits.split(id, split);
-  if (second && g.p.sorted) b = longest_first(a, b);
+  int own_len = 0;
+  if (second && g.p.sorted)
+    b = longest_first(a, b, own_len);
+  else if (!pooled)
+    own_len = __builtin_amdgcn_readfirstlane(sdpa_len(a, b));
   const int per_seq = a.q_len * a.group, nrows = pooled ? a.batch * per_seq : per_seq;
   const int row0 = tile * ROWS + (SHARED ? wave * 32 : 0);  // of this wave
-  const int own_len = pooled ? 0 : __builtin_amdgcn_readfirstlane(sdpa_len(a, b));
   // the tile's blocks: those of the prefix, then those of the sequence's own keys that its last row sees
   constexpr int bk = SHARED ? 32 * T::SB : 32;
   int own_n = 0;
@@ -516,6 +524,12 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   R.limit = 0;
   if (threadIdx.x == 0) sh.redo = sh.none = 0;
   __syncthreads();
+  // a few rows' own pages are asked for before Q: their loads return in order, and the first DMA needs them
+  Keys<DT, D, DR> ahead;
+  if constexpr (!SHARED) {
+    ahead = keys_of<DT, D, DR>(a, second, b, own_len, kvh);
+    if (ahead.table && split_first + wave < split_last) ahead.hold((split_first + wave) * 32);
+  }
   {
     const E* q = nullptr;
     if (row0 + (lane & 31) < nrows) {
@@ -531,7 +545,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   for (int seg = second; seg <= (int)(second || joint); ++seg) {
     const int first = seg ? std::max(split_first, np) - np : split_first, last = seg ? split_last - np : std::min(split_last, np);
     if (first >= last) continue;
-    Keys<DT, D, DR> S = keys_of<DT, D, DR>(a, seg, b, own_len, kvh);
+    Keys<DT, D, DR> S = SHARED ? keys_of<DT, D, DR>(a, seg, b, own_len, kvh) : ahead;
     const int all = seg ? 0 : a.prefix;  // keys that every query sees
     if constexpr (SHARED) {
       // Four waves of 32 rows over blocks of BK keys, two buffers for K and two for V.
