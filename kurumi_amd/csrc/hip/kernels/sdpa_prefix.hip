@@ -587,6 +587,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
 #pragma unroll
           for (int t = 0; t < T::SB; ++t) R.weigh(s[t], c, vbuf(par) + t * T::KT);
         }
+        __syncthreads();  // the next run's first block goes where this one's last may lie
       } else {
         // K runs one block ahead of V: the products of block blk + 1's scores, which are independent of
         // block blk's softmax, are issued between its exponentials, each fragment of K read two products

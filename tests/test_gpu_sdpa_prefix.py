@@ -133,6 +133,14 @@ def test_matches_the_definition(hip, dt, size):
 
 
 @pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("size", [(6, 182, 8, 2, 96, 30, 453, 16), (6, 182, 8, 2, 96, 30, 453, 0), (8, 128, 4, 2, 64, 20, 500, 8), (3, 200, 8, 4, 128, 95, 77, 0)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_tiles_whose_prefix_is_a_block_or_three(hip, dt, size):
+    """A tile goes from the prefix to the own keys after an odd number of blocks: its waves may be a block apart."""
+    Case(dt, *size[:7], page=size[7], lens=[size[6]] * size[0]).check(hip)
+
+
+@pytest.mark.parametrize("dt", FLOATS)
 def test_lengths_zero_one_and_past_the_range(hip, dt):
     """No own keys, one, fewer than queries; lengths outside [0, own_max] are taken into it."""
     print(f"sdpa_prefix lengths {dt.name}", flush=True)
