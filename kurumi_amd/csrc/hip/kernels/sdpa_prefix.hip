@@ -95,15 +95,11 @@ struct SdpaArgs {
 
 template <int DT>
 __device__ __forceinline__ void mfma_step(const u32x4& a, const u32x4& b, f32x16& c) {
-  if constexpr (DT == GT_BF16) {
+  static_assert(DT != GT_F32, "16-bit elements");
+  if constexpr (DT == GT_BF16)
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  } else if constexpr (DT == GT_F16) {
+  else
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  } else {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
-  }
 }
 
 template <int DT>
@@ -170,10 +166,12 @@ struct Rows {
       if (row && c < chunks) q[s] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(row) + c * 16);
     }
   }
-  // scores of 32 keys
+  // Scores of 32 keys. In f32 the products go into four sums: the error of a chain of d of them grows with
+  // its length, and a fourth of it halves the scores' error, which is most of the output's where keys are few.
   __device__ __forceinline__ f32x16 scores(const KU_LDS unsigned char* K) const {
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-    f32x16 s = {};
+    constexpr int SUMS = DT == GT_F32 ? 4 : 1;
+    f32x16 s[SUMS] = {};
     u32x4 k[3];  // fragments two steps ahead
     auto read = [&](int i) { return *(const KU_LDS u32x4*)(K + r * T::RB + (((2 * i + h) ^ T::kswz(r)) << 4)); };
     k[0] = read(0);
@@ -181,9 +179,18 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < T::DS; ++i) {
       if (i + 2 < T::DS) k[(i + 2) % 3] = read(i + 2);
-      mfma_step<DT>(k[i % 3], q[i], s);
+      if constexpr (DT == GT_F32) {
+        const f32x4 x = __builtin_bit_cast(f32x4, k[i % 3]), y = __builtin_bit_cast(f32x4, q[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], s[j], 0, 0, 0);
+      } else {
+        mfma_step<DT>(k[i % 3], q[i], s[0]);
+      }
     }
-    return s;
+    if constexpr (DT == GT_F32)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[0][v] = (s[0][v] + s[1][v]) + (s[2][v] + s[3][v]);
+    return s[0];
   }
   // keys from `left` on are not seen (left counts from the tile's first key)
   static __device__ __forceinline__ void mask(f32x16& s, int left) {
