@@ -429,7 +429,8 @@ size_t ku_hip_sdpa_prefix_scratch(const KuHipSdpaPrefixArgs *args);
  *          [0, vocab) are ignored. tokens NULL: no history.
  *   repetition (> 0), presence, frequency [rows] f32, each NULL for none
  *   bias_ids i32, bias_values f32 [bias_count], bias_offsets i32 [rows + 1]: row r has entries
- *          bias_offsets[r] to bias_offsets[r + 1] - 1 (taken into range). An id may repeat. NULL: none.
+ *          bias_offsets[r] to bias_offsets[r + 1] - 1 (taken into range). An id may repeat. NULL, or
+ *          bias_count 0: none.
  *   mask   [mask_rows, mask_stride words]: bit v % 32 of word v / 32 set = v is allowed. Row r goes by
  *          mask row mask_index[r] (mask_index NULL: r); an index outside [0, mask_rows) leaves the row
  *          unmasked. mask NULL: none.

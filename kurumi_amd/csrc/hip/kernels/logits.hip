@@ -252,11 +252,12 @@ void check_logits_adjust(const KuHipLogitsArgs& a) {
             "out overlaps logits without being the same");
   require(a.history <= kCount, "history is more than 2^30 - 1");
   if (a.tokens) span_of((int64_t)a.history, {{a.rows, a.tokens_stride}}, "tokens");
-  require(a.tokens || !(a.lens || a.prompt_lens), "lens or prompt_lens without tokens");
-  require((a.bias_ids != nullptr) == (a.bias_values != nullptr) && (a.bias_ids != nullptr) == (a.bias_offsets != nullptr),
+  // an array of no elements may be null beside others that are there
+  require(a.tokens || a.history == 0 || !(a.lens || a.prompt_lens), "lens or prompt_lens without tokens");
+  require(a.bias_count == 0 || ((a.bias_ids != nullptr) == (a.bias_values != nullptr) && (a.bias_ids != nullptr) == (a.bias_offsets != nullptr)),
           "bias_ids, bias_values and bias_offsets go together");
   require(a.bias_count <= 0x7fffffff, "bias_count is more than 2^31 - 1");
-  require(a.mask || !a.mask_index, "mask_index without mask");
+  require(a.mask || a.mask_rows == 0 || !a.mask_index, "mask_index without mask");
   if (a.mask) {
     require(a.mask_rows <= 0x7fffffff, "too many mask rows");
     require(a.mask_index || a.mask_rows >= a.rows, "fewer mask rows than rows, and no mask_index");

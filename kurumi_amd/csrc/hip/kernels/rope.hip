@@ -199,10 +199,12 @@ void check_rope(const KuHipRopeArgs& a) {
   require(std::isfinite(a.scale), "scale must be finite");
   require(a.tokens <= 0x7fffffff, "too many tokens");
   require(a.q_heads <= 16384 && a.kv_heads <= 16384, "too many heads");
-  require((a.q != nullptr) == (a.q_out != nullptr) && (a.k != nullptr) == (a.k_out != nullptr) &&
-              (a.v != nullptr) == (a.v_out != nullptr),
+  // of no tokens, an input may be null beside its output: the address of no elements
+  require(a.tokens == 0 ||
+              ((a.q != nullptr) == (a.q_out != nullptr) && (a.k != nullptr) == (a.k_out != nullptr) &&
+               (a.v != nullptr) == (a.v_out != nullptr)),
           "an input without its output, or an output without its input");
-  require(a.q || a.k || a.v, "nothing to do: q, k and v are all null");
+  require(a.tokens == 0 || a.q || a.k || a.v, "nothing to do: q, k and v are all null");
   require(!a.q || a.q_heads > 0, "q without q_heads");
   require(!(a.k || a.v) || a.kv_heads > 0, "k or v without kv_heads");
   if (a.rot_dim && (a.q || a.k)) {

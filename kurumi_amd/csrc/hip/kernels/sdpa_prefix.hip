@@ -1032,7 +1032,7 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
     strides16({a.prefix_row_stride, a.prefix_head_stride});
     span_of(d, {{a.prefix_len, a.prefix_row_stride}, {a.kv_heads, a.prefix_head_stride}}, "prefix_k");
   }
-  if (a.own_max) {
+  if (a.own_max && a.batch) {
     pointers16({a.own_k, a.own_v});
     require(a.own_lens, "own_max without own_lens");
     strides16({a.own_row_stride, a.own_head_stride});
@@ -1044,7 +1044,7 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
       require(a.pages_per_seq <= most && (__int128)a.pages_per_seq * a.page_size >= (__int128)a.own_max,
               "pages_per_seq pages do not hold own_max keys");
       require(a.own_rows / a.page_size >= 1 && a.own_rows / a.page_size <= most, "own_rows holds no page, or too many");
-    } else if (a.batch) {
+    } else {
       require(a.batch == 1 || a.own_seq_rows >= a.own_max, "own_seq_rows is less than own_max");
       require(a.own_seq_rows <= ((size_t)1 << 40) &&
                   (__int128)(a.batch - 1) * a.own_seq_rows + a.own_max <= (__int128)a.own_rows,

@@ -89,7 +89,8 @@ def rope_args(**kw):
 
 
 @pytest.mark.parametrize("kw", [
-    {}, dict(tokens=0), dict(rot_dim=0, freqs=None, positions=None), dict(q=None, q_out=None), dict(k=None, k_out=None, v=None, v_out=None),
+    {}, dict(tokens=0), dict(tokens=0, q=None, k=None, v=None, positions=None, rows=None), dict(tokens=0, q=None, q_out=None, k=None, v=None, rows=None),
+    dict(rot_dim=0, freqs=None, positions=None), dict(q=None, q_out=None), dict(k=None, k_out=None, v=None, v_out=None),
     dict(v=None, v_out=None), dict(rows=None), dict(q_out=2 * P, q_out_token_stride=512),  # in place
     dict(k_out=3 * P, k_out_row_stride=512, rows=None), dict(q_token_stride=0),  # a broadcast input
     dict(q_out_token_stride=64, q_out_head_stride=320),  # heads outermost
@@ -140,7 +141,7 @@ PAGED = dict(pages=9 * P, page_size=16, pages_per_seq=4)
 
 
 @pytest.mark.parametrize("kw", [
-    {}, dict(batch=0), dict(lse=None), dict(prefix_len=0, prefix_k=None, prefix_v=None), dict(own_max=0, own_lens=None, own_k=None, own_v=None),
+    {}, dict(batch=0), dict(batch=0, q=None, out=None, own_k=None, own_v=None, own_lens=None, pages=None, own_rows=0), dict(lse=None), dict(prefix_len=0, prefix_k=None, prefix_v=None), dict(own_max=0, own_lens=None, own_k=None, own_v=None),
     PAGED, dict(batch=1, own_seq_rows=0), dict(head_dim=8), dict(q_heads=2), dict(q_token_stride=0), dict(prefix_row_stride=0),
     dict(dtype=int(DType.F32), head_dim=4),
 ])
@@ -194,6 +195,9 @@ def logits_args(**kw):
     {}, dict(rows=0), dict(tokens=None, lens=None, prompt_lens=None), dict(mask=None, mask_index=None), dict(mask_index=None, mask_rows=4),
     dict(bias_ids=None, bias_values=None, bias_offsets=None), dict(tokens_stride=0), dict(logits_stride=0), dict(history=0),
     dict(out=P, out_dtype=int(DType.F16)), dict(repetition=None, presence=None, frequency=None), dict(lens=None, prompt_lens=None),
+    # what holds no elements may have no address
+    dict(bias_count=0, bias_ids=None, bias_values=None), dict(history=0, tokens=None), dict(mask_rows=0, mask=None),
+    dict(rows=0, logits=None, out=None, tokens=None, lens=None, prompt_lens=None, repetition=None),
 ])
 def test_logits_adjust_accepts(kw):
     assert accepted("ku_hip_logits_adjust", logits_args(**kw)), K.last_error()
