@@ -314,8 +314,9 @@ struct Keys {
     if (flat) return;
     const int lane = threadIdx.x & 63, r = lane / T::CPR;
     if (table) {
-      const int p1 = (j0 + KEYS - 1 < n ? j0 + KEYS - 1 : n - 1) >> shift;
-      if (held < 0 || p1 >= held + 64) hold(j0);
+      const int p0 = j0 >> shift, p1 = (j0 + KEYS - 1 < n ? j0 + KEYS - 1 : n - 1) >> shift;
+      // V is a block behind K: its pages too, where a wave has the lanes
+      if (held < 0 || p0 < held || p1 >= held + 64) hold(j0 >= KEYS && p1 < ((j0 - KEYS) >> shift) + 64 ? j0 - KEYS : j0);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         int j = j0 + (i * WAVES + wave) * RPD + r;

@@ -141,6 +141,13 @@ def test_tiles_whose_prefix_is_a_block_or_three(hip, dt, size):
 
 
 @pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("page", [1, 8])
+@pytest.mark.parametrize("size", [(32, 33, 16, 8, 32, 5, 1100), (64, 70, 4, 4, 128, 40, 600), (33, 104, 8, 8, 64, 5, 700)], ids=lambda s: "x".join(map(str, s)))
+def test_runs_of_more_pages_than_a_wave_has_lanes(hip, dt, size, page):
+    Case(dt, *size, page=page, lens=[size[6] - 7 * (b % 5) for b in range(size[0])]).check(hip)
+
+
+@pytest.mark.parametrize("dt", FLOATS)
 def test_lengths_zero_one_and_past_the_range(hip, dt):
     """No own keys, one, fewer than queries; lengths outside [0, own_max] are taken into it."""
     print(f"sdpa_prefix lengths {dt.name}", flush=True)
