@@ -255,18 +255,26 @@ struct Rows {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const float em = m == -INFINITY ? 0.f : -m;  // nothing seen so far: every score is -inf
     if constexpr (DT == GT_F32) {
+      // 32 keys in a sum of their own, which then joins O: a chain of every key's products would have an
+      // error that grows with the keys
       const int r = lane & 31;
+      float p[16];
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[v], c, em));
-        l += p;
-        const int key = (v >> 2) * 8 + (v & 3) + 4 * h;
+        p[v] = __builtin_amdgcn_exp2f(fmaf(s[v], c, em));
+        l += p[v];
+      }
 #pragma unroll
-        for (int t = 0; t < T::DTL; ++t) {
-          const int d = 32 * t + r;
+      for (int t = 0; t < T::DTL; ++t) {
+        f32x16 sum = {};
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int key = (v >> 2) * 8 + (v & 3) + 4 * h, d = 32 * t + r;
           const float x = *(const KU_LDS float*)(V + key * T::RB + (((d >> 2) ^ T::vswz(key)) << 4) + (d & 3) * 4);
-          o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p, o[t], 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[v], sum, 0, 0, 0);
         }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[t][v] += sum[v];
       }
     } else {
       u32x4 p[2];
