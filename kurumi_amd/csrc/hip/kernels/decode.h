@@ -85,6 +85,9 @@ inline bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
   return a < b + (uintptr_t)nq && b < a + (uintptr_t)np;
 }
 
+// work-groups of `threads` in one launch, whose threads are counted in 32 bits
+inline int64_t max_blocks(int threads) { return 0xffffffffll / threads; }
+
 inline void check_launch() {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) throw std::runtime_error(std::string("launch failed: ") + hipGetErrorString(e));

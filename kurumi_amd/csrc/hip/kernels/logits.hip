@@ -242,7 +242,8 @@ void check_logits_adjust(const KuHipLogitsArgs& a) {
   const int64_t w = (int64_t)float_width(a.dtype, "dtype"), wo = (int64_t)float_width(a.out_dtype, "out_dtype");
   require(a.rows <= 0x7fffffff, "too many rows");
   require(a.vocab >= 1 && a.vocab <= 0x7fffffff, "vocab must be 1 to 2^31 - 1");
-  require((__int128)((a.vocab + kThreads * kSmall - 1) / (kThreads * kSmall)) * a.rows <= 0x7fffffff, "too many rows of this vocab");
+  // so many rows take large chunks
+  require((__int128)((a.vocab + kThreads * kLarge - 1) / (kThreads * kLarge)) * a.rows <= max_blocks(kThreads), "too many rows of this vocab");
   require((a.logits && a.out) || a.rows == 0, "null logits or out");
   require(aligned_to(a.logits, (size_t)w) && aligned_to(a.out, (size_t)wo), "pointers must be aligned to their elements");
   const int64_t ni = span_of((int64_t)a.vocab, {{a.rows, a.logits_stride}}, "logits") * w;

@@ -54,7 +54,8 @@ template <> struct Bits<16> { using T = uint4; };
 // layout: i and i + rot / 2; interleaved: next to each other), or up to two vectors that are copied.
 // A work-group takes block_tokens tokens; it forms their angles once, in LDS, for all heads: a sine and
 // cosine of a 64-bit angle for each unit of each head would take longer than moving the unit.
-// 8192 tokens of 48 heads of 128, bf16: see the table of the kernel's cases.
+// Bound by memory: 8192 tokens of 48 heads of 128, bf16, with the store (201 MB in and out), 40.2 us, 5.0 TB/s,
+// where a copy of 1 GiB reaches 5.06; 16 tokens 3.6 us, a launch.
 template <int DT, class T, int V, bool HALF>
 __global__ void __launch_bounds__(kThreads) rope_k(RopeDev a) {
   using W = typename Bits<V * (int)sizeof(T)>::T;
@@ -140,27 +141,76 @@ __global__ void __launch_bounds__(kThreads) rope_k(RopeDev a) {
   }
 }
 
-template <int DT, class T, int V>
-void launch_v(RopeDev& d, uint32_t q_heads, uint32_t k_heads, uint32_t v_heads, bool half, hipStream_t s) {
-  auto units = [](uint32_t features) { return (features + 2 * V - 1) / (2 * V); };
-  d.turned = d.rot / 2 / V;
+// How a call runs: V elements at a time, the kernel's arguments and its launch.
+struct RopePlan {
+  RopeDev d;
+  int v = 1;
+  dim3 grid;
+  size_t lds = 0;
+};
+
+RopePlan make_plan(const KuHipRopeArgs& a) {
+  RopePlan p;
+  RopeDev& d = p.d;
+  d.q = {a.q, a.q_out, a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride};
+  d.k = {a.k, a.k_out, a.k_token_stride, a.k_head_stride, a.k_out_row_stride, a.k_out_head_stride};
+  d.v = {a.v, a.v_out, a.v_token_stride, a.v_head_stride, a.v_out_row_stride, a.v_out_head_stride};
+  d.positions = a.positions;
+  d.rows = a.rows;
+  d.tokens = (int64_t)a.tokens;
+  d.out_rows = (int64_t)a.out_rows;
+  d.dim = (uint32_t)a.head_dim;
+  d.rot = a.q || a.k ? (uint32_t)a.rot_dim : 0;
+  d.scale = a.scale;
+  for (uint32_t i = 0; i < d.rot / 2; ++i) d.turns[i] = (a.inverse ? -a.freqs[i] : a.freqs[i]) / 6.283185307179586476925;
+  const uint32_t qh = a.q ? (uint32_t)a.q_heads : 0, kh = a.k ? (uint32_t)a.kv_heads : 0, vh = a.v ? (uint32_t)a.kv_heads : 0;
+  // as many bytes at a time, up to 16, as everything is made of
+  const size_t width = a.dtype == KU_F32 ? 4 : 2;
+  auto made_of = [&](int64_t v) {
+    bool ok = d.dim % v == 0 && (d.rot / 2) % v == 0;
+    for (const RopeSide* x : {&d.q, &d.k, &d.v})
+      if (x->in)
+        ok = ok && aligned_to(x->in, v * width) && aligned_to(x->out, v * width) && x->in_token % v == 0 && x->in_head % v == 0 &&
+             x->out_row % v == 0 && x->out_head % v == 0;
+    return ok;
+  };
+  p.v = 16 / (int)width;
+  while (p.v > 1 && !made_of(p.v)) p.v /= 2;
+  auto units = [&](uint32_t features) { return (features + 2 * p.v - 1) / (2 * p.v); };
+  d.turned = d.rot / 2 / p.v;
   d.copied = units(d.dim - d.rot);
   d.v_units = units(d.dim);
-  d.q_units = q_heads * (d.turned + d.copied);
-  d.qk_units = d.q_units + k_heads * (d.turned + d.copied);
-  d.units = d.qk_units + v_heads * d.v_units;
+  d.q_units = qh * (d.turned + d.copied);
+  d.qk_units = d.q_units + kh * (d.turned + d.copied);
+  d.units = d.qk_units + vh * d.v_units;
   // Work-groups of about two units a thread where that leaves enough of them (8192 tokens of 48 heads of
   // 128, bf16: 41.8 us; 47 with eight a thread, 56 with four of those in flight), of one where it does not:
   // a few tokens are spread over their heads.
   const int64_t all = d.tokens * (int64_t)d.units, want = all / (2 * kThreads) >= 4 * (int64_t)cu_count() ? 2 * kThreads : kThreads;
   d.block_tokens = (uint32_t)std::max<int64_t>(1, std::min<int64_t>({want / d.units, d.tokens, 64}));
   d.block_units = d.block_tokens > 1 ? d.units : (uint32_t)std::min<int64_t>(d.units, std::max<int64_t>(want, (d.units + 65534) / 65535));
-  const dim3 grid((unsigned)((d.tokens + d.block_tokens - 1) / d.block_tokens), (d.units + d.block_units - 1) / d.block_units);
-  const size_t lds = d.block_tokens * (d.rot / 2) * sizeof(float2);
+  p.grid = dim3((unsigned)((d.tokens + d.block_tokens - 1) / d.block_tokens), (d.units + d.block_units - 1) / d.block_units);
+  p.lds = d.block_tokens * (d.rot / 2) * sizeof(float2);
+  return p;
+}
+
+template <int DT, class T, int V>
+void launch_v(const RopePlan& p, bool half, hipStream_t s) {
   if (half)
-    hipLaunchKernelGGL((rope_k<DT, T, V, true>), grid, dim3(kThreads), lds, s, d);
+    hipLaunchKernelGGL((rope_k<DT, T, V, true>), p.grid, dim3(kThreads), p.lds, s, p.d);
   else
-    hipLaunchKernelGGL((rope_k<DT, T, V, false>), grid, dim3(kThreads), lds, s, d);
+    hipLaunchKernelGGL((rope_k<DT, T, V, false>), p.grid, dim3(kThreads), p.lds, s, p.d);
+}
+template <int DT, class T>
+void launch_t(const RopePlan& p, bool half, hipStream_t s) {
+  switch (p.v) {
+    case 8:
+      if constexpr (sizeof(T) == 2) launch_v<DT, T, 8>(p, half, s);
+      break;
+    case 4: launch_v<DT, T, 4>(p, half, s); break;
+    case 2: launch_v<DT, T, 2>(p, half, s); break;
+    default: launch_v<DT, T, 1>(p, half, s); break;
+  }
 }
 
 }  // namespace
@@ -233,50 +283,20 @@ void check_rope(const KuHipRopeArgs& a) {
        a.rows != nullptr, "k or k_out");
   side(a.v, a.v_token_stride, a.v_head_stride, a.v_out, a.v_out_row_stride, a.v_out_head_stride, a.kv_heads, a.out_rows,
        a.rows != nullptr, "v or v_out");
+  if (a.tokens) {
+    const dim3 grid = make_plan(a).grid;
+    require((int64_t)grid.x * grid.y <= max_blocks(kThreads), "too many tokens for one launch");
+  }
 }
 
 void launch_rope(const KuHipRopeArgs& a, hipStream_t s) {
   if (a.tokens == 0) return;
-  RopeDev d;
-  d.q = {a.q, a.q_out, a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride};
-  d.k = {a.k, a.k_out, a.k_token_stride, a.k_head_stride, a.k_out_row_stride, a.k_out_head_stride};
-  d.v = {a.v, a.v_out, a.v_token_stride, a.v_head_stride, a.v_out_row_stride, a.v_out_head_stride};
-  d.positions = a.positions;
-  d.rows = a.rows;
-  d.tokens = (int64_t)a.tokens;
-  d.out_rows = (int64_t)a.out_rows;
-  d.dim = (uint32_t)a.head_dim;
-  d.rot = a.q || a.k ? (uint32_t)a.rot_dim : 0;
-  d.scale = a.scale;
-  for (uint32_t i = 0; i < d.rot / 2; ++i) d.turns[i] = (a.inverse ? -a.freqs[i] : a.freqs[i]) / 6.283185307179586476925;
-  const uint32_t qh = a.q ? (uint32_t)a.q_heads : 0, kh = a.k ? (uint32_t)a.kv_heads : 0, vh = a.v ? (uint32_t)a.kv_heads : 0;
+  const RopePlan p = make_plan(a);
   const bool half = a.layout == KU_ROPE_HALF;
-  // as many bytes at a time, up to 16, as everything is made of
-  auto made_of = [&](int64_t v) {
-    bool ok = d.dim % v == 0 && (d.rot / 2) % v == 0;
-    const size_t bytes = (size_t)v * (a.dtype == KU_F32 ? 4 : 2);
-    for (const RopeSide* x : {&d.q, &d.k, &d.v})
-      if (x->in)
-        ok = ok && aligned_to(x->in, bytes) && aligned_to(x->out, bytes) && x->in_token % v == 0 && x->in_head % v == 0 &&
-             x->out_row % v == 0 && x->out_head % v == 0;
-    return ok;
-  };
-  auto go = [&](auto dt, auto elem) {
-    constexpr int DT = decltype(dt)::value;
-    using T = decltype(elem);
-    if (sizeof(T) == 2 && made_of(8))
-      launch_v<DT, T, sizeof(T) == 2 ? 8 : 4>(d, qh, kh, vh, half, s);
-    else if (made_of(4))
-      launch_v<DT, T, 4>(d, qh, kh, vh, half, s);
-    else if (made_of(2))
-      launch_v<DT, T, 2>(d, qh, kh, vh, half, s);
-    else
-      launch_v<DT, T, 1>(d, qh, kh, vh, half, s);
-  };
   switch (a.dtype) {
-    case KU_BF16: go(DTag<GT_BF16>{}, uint16_t{}); break;
-    case KU_F16: go(DTag<GT_F16>{}, uint16_t{}); break;
-    default: go(DTag<GT_F32>{}, float{}); break;
+    case KU_BF16: launch_t<GT_BF16, uint16_t>(p, half, s); break;
+    case KU_F16: launch_t<GT_F16, uint16_t>(p, half, s); break;
+    default: launch_t<GT_F32, float>(p, half, s); break;
   }
   check_launch();
 }

@@ -978,18 +978,25 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
 
 int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
+int64_t tile_groups(const SdpaPlan& p) {
+  return 8 * (((int64_t)p.part[0].units + 7) / 8 + ((int64_t)p.part[1].units + 7) / 8);
+}
+// Few slots: several rows a wave (32768 rows of 64, two slots: 7.2 us, and 14 with a wave a row).
+int64_t join_groups(int64_t rows, int slots, int d) {
+  const int64_t each = 4 * (slots <= 8 ? 256 / d : 1);
+  return slots == 1 ? 0 : (rows + each - 1) / each;
+}
+
 template <int DT, int D, int DR>
 void launch_d(const SdpaArgs& g, hipStream_t s) {
-  const unsigned groups = 8 * (unsigned)((g.p.part[0].units + 7) / 8 + (g.p.part[1].units + 7) / 8);
+  const unsigned groups = (unsigned)tile_groups(g.p);
   if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR>), dim3(groups), dim3(256), 0, s, g);
-  const int64_t rows = (int64_t)g.a.batch * g.a.q_len * g.a.q_heads;
-  if (g.p.slots == 1) return;
-  // few slots: several rows a wave (32768 rows of 64, two slots: 14 us with a wave a row)
-  constexpr int S = 256 / D;
+  const unsigned joins = (unsigned)join_groups((int64_t)g.a.batch * g.a.q_len * g.a.q_heads, g.p.slots, D);
+  if (joins == 0) return;
   if (g.p.slots <= 8)
-    hipLaunchKernelGGL((sdpa_join_k<DT, D, 1>), dim3((unsigned)((rows + 4 * S - 1) / (4 * S))), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((sdpa_join_k<DT, D, 1>), dim3(joins), dim3(256), 0, s, g);
   else
-    hipLaunchKernelGGL((sdpa_join_k<DT, D, S>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((sdpa_join_k<DT, D, 256 / D>), dim3(joins), dim3(256), 0, s, g);
 }
 template <int DT>
 void launch_t(const SdpaArgs& g, int d, hipStream_t s) {
@@ -1059,6 +1066,11 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
                   (__int128)(a.batch - 1) * a.own_seq_rows + a.own_max <= (__int128)a.own_rows,
               "own_rows does not hold own_max keys of every sequence");
     }
+  }
+  if (a.batch) {
+    const SdpaPlan p = make_plan(a);
+    require(tile_groups(p) <= max_blocks(256) && join_groups(a.batch * a.q_len * a.q_heads, p.slots, padded_dim(a.head_dim)) <= max_blocks(256),
+            "more queries than one launch takes");
   }
 }
 

@@ -111,6 +111,8 @@ def test_rope_accepts(kw):
     (dict(q_out_head_stride=63), "overlap"), (dict(q_out_token_stride=255), "overlap"), (dict(k_out_row_stride=0), "overlap"),
     (dict(q_out=2 * P + 128), "overlaps its input"), (dict(q_out=2 * P), "overlaps its input"),
     (dict(k_out=3 * P, k_out_row_stride=512), "no rows"), (dict(q_token_stride=1 << 62), "address space"),
+    (dict(tokens=(1 << 31) - 1, head_dim=2, rot_dim=0, q_heads=1, q_head_stride=0, q_token_stride=2, q_out_head_stride=0, q_out_token_stride=2,
+          k=None, k_out=None, v=None, v_out=None, q_out=1 << 40), "one launch"),
 ])
 def test_rope_refusals(kw, what):
     assert re.search(what, said("ku_hip_rope", rope_args(**kw)))
@@ -162,6 +164,8 @@ def test_sdpa_prefix_accepts(kw):
     (dict(out_token_stride=0), "overlap"), (dict(out=P), "out overlaps q"), (dict(out=P + 512), "out overlaps q"),
     (dict(own_seq_rows=49), "own_seq_rows"), (dict(own_rows=149), "own_rows does not hold"), (dict(q_batch_stride=-1024), "negative"),
     ({**PAGED, "page_size": 12}, "power of two"), ({**PAGED, "page_size": 0}, "power of two"), ({**PAGED, "pages_per_seq": 3}, "pages_per_seq"),
+    (dict(batch=1 << 20, q_len=1, q_heads=64, kv_heads=64, head_dim=8, q_batch_stride=512, q_head_stride=8, out_batch_stride=512,
+          out_head_stride=8, out=1 << 42, own_max=1, own_rows=1 << 20, own_seq_rows=1), "one launch"),
     ({**PAGED, "own_rows": 15}, "no page"), ({**PAGED, "pages": 9 * P + 2}, "4-byte aligned"),
 ])
 def test_sdpa_prefix_refusals(kw, what):
@@ -211,6 +215,7 @@ def test_logits_adjust_accepts(kw):
     (dict(bias_ids=None), "go together"), (dict(bias_offsets=None), "go together"), (dict(bias_count=1 << 31), "bias_count"),
     (dict(mask=None), "mask_index without mask"), (dict(mask_index=None), "fewer mask rows"), (dict(mask_stride=-1), "negative"),
     (dict(tokens=3 * P + 2), "aligned"), (dict(mask=12 * P + 1), "aligned"), (dict(rows=1 << 40), "too many|address space"),
+    (dict(rows=1 << 24), "too many rows"),
 ])
 def test_logits_adjust_refusals(kw, what):
     assert re.search(what, said("ku_hip_logits_adjust", logits_args(**kw)))
