@@ -23,6 +23,14 @@
 // behind them cannot matter. A query whose sums are not finite, or that saw nothing, is done again from
 // the definition by sdpa_one: an infinity or NaN in a value that another query of the tile sees, and a
 // page that is none, come out right that way.
+//
+// What bounds it, 32 heads over 8 of 128 features, us of both kernels:
+//   1 query each of 32 sequences, 65536 shared keys, f16 (303 MB): 78, 3.9 TB/s; the loop alone runs at the
+//     rate of a copy (5 TB/s), the rest is a unit's start, its partial result and the join
+//   64 sequences of up to 1024 own keys in pages of 16 beside 8192 shared ones, bf16 (171 MB): 50, 3.4 TB/s;
+//     the own keys, which few work-groups read with little in flight at the end
+//   256 queries each of 8 sequences, 16 heads over 4 of 64, 4096 shared keys, bf16 (37 GFLOP): 61, 0.6 PFLOP/s;
+//     the vector units: over 64 features a score's exponential and sums take as long as its two products
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -434,8 +442,9 @@ __device__ __forceinline__ bool unit_of(const SdpaPlan& p, int i, bool& second, 
 }
 
 // The sequence of a batch of up to 64 that unit position i of the own keys takes: the longest first, so that
-// the last work-groups to start are the shortest (64 sequences of 16 to 1024 keys beside 8192 shared ones:
-// see the table), and by turns over the XCDs, each of which has a run of positions.
+// the last work-groups to start are the shortest, and by turns over the XCDs, each of which has a run of
+// positions. 64 sequences of 16 to 1024 keys beside 8192 shared ones: 44.8 us, 49.4 in their own order; 32
+// sequences 26.3 and 28.2; 16 queries each of 32 sequences 34.3 and 39.1.
 __device__ __forceinline__ int longest_first(const SdpaDev& a, int i, int& len) {
   const int lane = threadIdx.x & 63, n = a.batch;
   const int g = n & 7 ? (n & 3 ? (n & 1 ? 1 : 2) : 4) : 8, period = n / g;
@@ -944,9 +953,9 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
   auto cut = [&](SdpaPlan::Part& part, int64_t rows, int64_t items, int64_t keys, int64_t want) {
     if (keys == 0 || items == 0 || rows == 0) return;
     // Tiles of 128 rows read a key once where four tiles of 32 read it four times (from L2, and with every
-    // wave's own DMA); tiles of 32 spread few rows' keys over all four waves. us of the kernel, bf16, 32
-    // heads over 8 of 128, 8192 shared keys: 48 rows 14.5 / 13.0, 96 rows 27.8 / 25.8 (own keys among
-    // them); 65536 keys: 64 rows 68 / 67, 128 rows 65.6 / 88.9.
+    // wave's own DMA); tiles of 32 spread few rows' keys over all four waves. us of both kernels, 128 / 32
+    // rows, bf16, 32 heads over 8 of 128, 8192 shared keys: 48 rows 19.8 / 17.4, 96 rows 22.1 / 21.2, 128 rows
+    // 31.9 / 34.9; 65536 keys: 64 rows 71.6 / 72.7, 128 rows 79.3 / 112.
     part.shared = rows > 64;
     part.tiles = (int)((rows + (part.shared ? 127 : 31)) / (part.shared ? 128 : 32));
     const int64_t bk = part.shared ? (a.dtype == KU_F32 ? 32 : 64) : 128, blocks = (keys + bk - 1) / bk;
@@ -959,9 +968,10 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     cut(p.part[0], per_seq, nb * kv, (int64_t)(a.prefix_len + a.own_max), 2 * cu);
   } else {
     // A unit costs about 4 us before its first product and 3 to write its partial result, so more of them
-    // than CUs lose: the prefix alone 22.5 us with one a CU, 28 with two, 31 with one for two CUs (256 rows,
-    // 8192 keys). Beside own keys of half its length or more it leaves every other CU to them: 49 us, and 55
-    // with one a CU (64 sequences of up to 1024 own keys).
+    // than CUs lose: the prefix alone 30 us with one a CU, 38 with two and 38 with one for two CUs (256 rows,
+    // 8192 keys), 79 / 93 / 110 (128 rows, 65536 keys). Beside own keys of half its length or more it leaves
+    // every other CU to them: 50 us, and 55 with one a CU (64 sequences of up to 1024 own keys), 31 and 37
+    // (32 sequences).
     cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len, nb * (int64_t)a.own_max * 2 >= (int64_t)a.prefix_len ? cu / 2 : cu);
     cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max, 2 * cu);
   }
