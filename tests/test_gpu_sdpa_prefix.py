@@ -336,6 +336,14 @@ def test_a_batch_without_sequences_and_one_head_of_outputs(hip):
     np.testing.assert_array_equal(o1, o2)
 
 
+@pytest.mark.parametrize("dt", FLOATS)
+def test_no_keys_at_all(hip, dt):
+    c = Case(dt, 5, 2, 6, 3, 72, 0, 0)
+    assert K.sdpa_prefix_scratch(c.args()) == 0
+    o, lse = c.run(hip)
+    assert (o == 0).all() and (lse == -np.inf).all()
+
+
 def test_own_cache_past_2_to_32_elements(hip):
     """A cache of 8 GiB a tensor: the last page and the last sequence lie past 2^32 elements."""
     kv, d, page = 8, 128, 16
