@@ -950,7 +950,7 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
   // One sequence's rows walk the prefix by themselves where they fill tiles of 128 to four fifths; else
   // the sequences' rows share tiles over it.
   p.joint = (per_seq + 127) / 128 * 128 * 4 <= per_seq * 5;
-  auto cut = [&](SdpaPlan::Part& part, int64_t rows, int64_t items, int64_t keys, int64_t want) {
+  auto cut = [&](SdpaPlan::Part& part, int64_t rows, int64_t items, int64_t keys, int64_t want, bool halves = false) {
     if (keys == 0 || items == 0 || rows == 0) return;
     // Tiles of 128 rows read a key once where four tiles of 32 read it four times (from L2, and with every
     // wave's own DMA); tiles of 32 spread few rows' keys over all four waves. us of both kernels, 128 / 32
@@ -959,7 +959,8 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     part.shared = rows > 64;
     part.tiles = (int)((rows + (part.shared ? 127 : 31)) / (part.shared ? 128 : 32));
     const int64_t bk = part.shared ? (a.dtype == KU_F32 ? 32 : 64) : 128, blocks = (keys + bk - 1) / bk;
-    part.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want / (items * part.tiles), blocks, 256}));
+    const int64_t least = halves && items * part.tiles <= cu ? 2 : 1;
+    part.splits = (int)std::max<int64_t>(1, std::min<int64_t>({std::max(want / (items * part.tiles), least), blocks, 256}));
     part.units = (int)(items * part.tiles * part.splits);
     part.by_tiles = Div(part.tiles);
     part.by_splits = Div(part.splits);
@@ -972,8 +973,14 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     // 8192 keys), 79 / 93 / 110 (128 rows, 65536 keys). Beside own keys of half its length or more it leaves
     // every other CU to them: 50 us, and 55 with one a CU (64 sequences of up to 1024 own keys), 31 and 37
     // (32 sequences).
-    cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len, nb * (int64_t)a.own_max * 2 >= (int64_t)a.prefix_len ? cu / 2 : cu);
-    cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max, 2 * cu);
+    const bool beside = nb * (int64_t)a.own_max * 2 >= (int64_t)a.prefix_len;
+    cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len, beside ? cu / 2 : cu);
+    // Own keys: a unit a CU, but halves where each sequence would be one unit and every CU had at most one,
+    // unless the prefix outlasts them. us of the tiles with cu / 2 cu units wanted, bf16, 8192 shared and up to
+    // 1024 own keys: 4 sequences 13.0 / 13.0, 8 15.5 / 17.0, 16 19.7 / 20.0; halves 32 sequences 26.0, whole 29.9;
+    // 4 sequences of up to 8192 27.9 / 32.7, one 11.8 / 14.2; under 65536 shared keys (32 sequences) 71.3 / 73.0;
+    // quarters cost 64 sequences 50 where they take 43.5.
+    cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max, cu, beside);
   }
   p.slots = p.part[0].splits + p.part[1].splits;
   // keys fit 25 bits beside a lane's number; one round of work-groups needs no order
