@@ -25,7 +25,7 @@
 // page that is none, come out right that way.
 //
 // What bounds it, 32 heads over 8 of 128 features, us of both kernels:
-//   1 query each of 32 sequences, 65536 shared keys, f16 (303 MB): 78, 3.9 TB/s; the loop alone runs at the
+//   1 query each of 32 sequences, 65536 shared keys, f16 (303 MB): 77, 3.9 TB/s; the loop alone runs at the
 //     rate of a copy (5 TB/s), the rest is a unit's start, its partial result and the join
 //   64 sequences of up to 1024 own keys in pages of 16 beside 8192 shared ones, bf16 (171 MB): 50, 3.4 TB/s;
 //     the own keys, which few work-groups read with little in flight at the end
@@ -966,6 +966,8 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     part.by_splits = Div(part.splits);
   };
   if (p.joint) {
+    // two a CU, so that one's products meet the other's exponentials: 256 queries each of 4 sequences on 4096
+    // shared keys, 16 heads over 4 of 128, 50 us and 64 with one; of one sequence 25 and 27
     cut(p.part[0], per_seq, nb * kv, (int64_t)(a.prefix_len + a.own_max), 2 * cu);
   } else {
     // A unit costs about 4 us before its first product and 3 to write its partial result, so more of them
