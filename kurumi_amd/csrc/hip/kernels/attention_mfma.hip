@@ -33,6 +33,7 @@
 #include "kernels.h"
 #include "lds_dma.h"
 #include "numeric.h"
+#include "pair16.h"
 
 namespace ku::hipbk {
 
@@ -43,9 +44,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((__vector_size__(4 * sizeof(short))));
 #define KU_LDS __attribute__((address_space(3)))
 
@@ -60,39 +58,6 @@ __device__ __forceinline__ f32x16 mfma(const u32x4& a, const u32x4& b, const f32
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                   0, 0);
-}
-
-// two f32 -> one dword of two 16-bit values, rounded to nearest even by v_cvt_pk_bf16_f32 /
-// v_cvt_f16_f32 (the probabilities and outputs here are never NaN unless an input is)
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const f32x2 v = {lo, hi};
-  if constexpr (DT == GT_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-}
-
-// c + lo + hi of a packed pair of 16-bit floats (v_dot2c_f32_{bf16,f16} against 1.0 pairs)
-template <int DT>
-__device__ __forceinline__ float sum2(uint32_t pair, float c) {
-  if constexpr (DT == GT_BF16) {
-    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), one, c, false);
-  } else {
-    const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), one, c, false);
-  }
-}
-
-// the two values of a packed pair
-template <int DT>
-__device__ __forceinline__ float lower(uint32_t pair) {
-  if constexpr (DT == GT_BF16) return __uint_as_float(pair << 16);
-  else return (float)__builtin_bit_cast(f16x2, pair)[0];
-}
-template <int DT>
-__device__ __forceinline__ float upper(uint32_t pair) {
-  if constexpr (DT == GT_BF16) return __uint_as_float(pair & 0xffff0000u);
-  else return (float)__builtin_bit_cast(f16x2, pair)[1];
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, uint32_t bytes) {

@@ -15,7 +15,7 @@
 // + v % 4, so maximum, sum and rescale are a lane's own scalars, and the probabilities lie in registers
 // as the second product's operand. K and V go to LDS by DMA.
 //
-// The keys of a tile are cut into splits until the chip is full; each split leaves its maximum, sum and
+// The keys of a tile are cut into splits until the chip is full; each split leaves its maximum, sums and
 // unnormalised output in f32 in the scratch and a second kernel joins them in split order. A tile with
 // one split writes its output itself.
 //
@@ -39,6 +39,7 @@
 
 #include "decode.h"
 #include "lds_dma.h"
+#include "pair16.h"
 #include "sdpa_prefix.h"
 
 namespace ku::hipbk {
@@ -49,11 +50,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((__vector_size__(4 * sizeof(short))));
 #define KU_LDS __attribute__((address_space(3)))
 
@@ -98,7 +96,7 @@ struct SdpaArgs {
   SdpaDev a;
   SdpaPlan p;
   float* po;   // [rows][slots][D]
-  float2* ml;  // [rows][slots]: maximum in powers of two, sum
+  float4* ml;  // [rows][slots]: maximum in powers of two, sum, sum of the probabilities before rounding
 };
 
 template <int DT>
@@ -110,12 +108,6 @@ __device__ __forceinline__ void mfma_step(const u32x4& a, const u32x4& b, f32x16
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const f32x2 v = {lo, hi};
-  if constexpr (DT == GT_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-}
 // the value of the other half of the wave
 __device__ __forceinline__ float other_half(float x) {
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -148,17 +140,23 @@ struct Tile {
 };
 
 // One wave's 32 rows of a tile: Q fragments, running maximum, sum and O.
-template <int DT, int D, int DR>
+//
+// Probabilities of 16-bit keys are rounded to 16 bits for the second product, and the output is divided by the sum
+// of the rounded ones: where many round the same way, a mean with unrounded ones below would be off by that rounding.
+// lse is of the unrounded sum, which is formed where it is asked for (LSE).
+template <int DT, int D, int DR, bool LSE>
 struct Rows {
   using T = Tile<DT, D, DR>;
+  static constexpr bool WHOLE = LSE && DT != GT_F32;  // two sums
   u32x4 q[T::DS];
   f32x16 o[T::DTL];
   float m, l;  // m in powers of two, already times scale
+  float w;     // WHOLE: the sum before rounding
   int limit;   // own keys that this lane's query sees
 
   __device__ __forceinline__ void clear() {
     m = -INFINITY;
-    l = 0.f;
+    l = w = 0.f;
 #pragma unroll
     for (int t = 0; t < T::DTL; ++t)
 #pragma unroll
@@ -200,6 +198,21 @@ struct Rows {
       for (int v = 0; v < 16; ++v) s[0][v] = (s[0][v] + s[1][v]) + (s[2][v] + s[3][v]);
     return s[0];
   }
+  // Sums of a block's probabilities of 16 bits, in two chains.
+  struct Sums {
+    float l[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
+    // two probabilities as the product takes them
+    __device__ __forceinline__ uint32_t add(int i, float p0, float p1) {
+      const uint32_t pp = pack2<DT>(p0, p1);
+      l[i] = sum2<DT>(pp, l[i]);
+      if constexpr (WHOLE) w[i] += p0 + p1;
+      return pp;
+    }
+  };
+  __device__ __forceinline__ void join(const Sums& r) {
+    l += r.l[0] + r.l[1];
+    if constexpr (WHOLE) w += r.w[0] + r.w[1];
+  }
   // keys from `left` on are not seen (left counts from the tile's first key)
   static __device__ __forceinline__ void mask(f32x16& s, int left) {
     const int lim = left - 4 * ((threadIdx.x & 63) >> 5);
@@ -221,6 +234,7 @@ struct Rows {
       const float mn = need ? bm : m, corr = need ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
       m = mn;
       l *= corr;
+      if constexpr (WHOLE) w *= corr;
 #pragma unroll
       for (int t = 0; t < T::DTL; ++t)
 #pragma unroll
@@ -257,8 +271,7 @@ struct Rows {
       for (int t = 0; t < T::DTL; ++t) mfma_step<DT>(f[st & 1][t], p[st], o[t]);
     }
   }
-  // O^T += V^T P^T over 32 keys. The product takes probabilities rounded to the 16 bits of V, half a step
-  // each (the output's own rounding is one more); their sum, which lse is made of, stays in f32.
+  // O^T += V^T P^T over 32 keys, with the probabilities' sums.
   __device__ __forceinline__ void weigh(const f32x16& s, float c, const KU_LDS unsigned char* V) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const float em = m == -INFINITY ? 0.f : -m;  // nothing seen so far: every score is -inf
@@ -286,16 +299,14 @@ struct Rows {
       }
     } else {
       u32x4 p[2];
-      float rs[2] = {0.f, 0.f};
+      Sums r;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * i], c, em));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], c, em));
-        const uint32_t pp = pack2<DT>(p0, p1);
-        rs[i & 1] += p0 + p1;
-        p[i >> 2][i & 3] = pp;
+        p[i >> 2][i & 3] = r.add(i & 1, p0, p1);
       }
-      l += rs[0] + rs[1];
+      join(r);
       product(p, V);
     }
   }
@@ -502,13 +513,13 @@ __device__ __forceinline__ void touch_arguments() {
 
 // LDS of a work-group beside the tiles of keys.
 struct SdpaShared {
-  float2 ml[4][32];
+  float4 ml[4][32];
   uint32_t redo, none;
 };
 
 // One unit: a tile of rows against a split of its keys. SHARED: four waves of 32 rows share blocks of
 // keys; else the waves deal the blocks of one tile of 32 rows among them.
-template <int DT, int D, int DR, bool SHARED>
+template <int DT, int D, int DR, bool LSE, bool SHARED>
 __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id, unsigned char* lds_raw, SdpaShared& sh) {
   using T = Tile<DT, D, DR>;
   using E = typename SdpaElem<DT>::T;
@@ -544,7 +555,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   int split_first, split_last;
   split_range(part.by_splits, np + no, split, split_first, split_last);
   bool none = false;
-  Rows<DT, D, DR> R;
+  Rows<DT, D, DR, LSE> R;
   R.clear();
   R.limit = 0;
   if (threadIdx.x == 0) sh.redo = sh.none = 0;
@@ -629,7 +640,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
             R.rescale(sc, c);
             const float em = R.m == -INFINITY ? 0.f : -R.m;
             u32x4 p[4];
-            float rs[2] = {0.f, 0.f};
+            typename Rows<DT, D, DR, LSE>::Sums rs;
             const int r = lane & 31;
             const KU_LDS unsigned char* LK = kbuf(PAR ^ 1);
             auto kread = [&](int m) {
@@ -647,16 +658,14 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
                 const int te = i >> 3, v2 = i & 7;
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2], c, em));
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2 + 1], c, em));
-                const uint32_t pp = pack2<DT>(p0, p1);
-                rs[v2 & 1] += p0 + p1;  // unrounded: the sum is an output too
-                p[2 * te + (v2 >> 2)][v2 & 3] = pp;
+                p[2 * te + (v2 >> 2)][v2 & 3] = rs.add(v2 & 1, p0, p1);
               }
               if (m < 2) sn[m & 1] = f32x16{};
               mfma_step<DT>(kf[m % 3], R.q[m >> 1], sn[m & 1]);
               __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_setprio(0);
-            R.l += rs[0] + rs[1];
+            R.join(rs);
             R.product(p, vbuf(PAR));
           }
           vm_wait<0>();
@@ -728,6 +737,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   const bool there = row0 + (lane & 31) < nrows;
   const int slots = g.p.slots, slot = second ? g.p.part[0].splits + split : split;
   R.l += other_half(R.l);
+  R.w = Rows<DT, D, DR, LSE>::WHOLE ? R.w + other_half(R.w) : R.l;
   if (__builtin_amdgcn_ballot_w64(none) != 0 && lane == 0) atomicOr(&sh.none, 1u);
   uint32_t redo = 0;  // rows of this wave that are done again
   __syncthreads();
@@ -744,7 +754,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
           for (int v = 0; v < 4; ++v)
             *reinterpret_cast<f32x4*>(o + 32 * t + 8 * v + 4 * h) =
                 f32x4{R.o[t][4 * v], R.o[t][4 * v + 1], R.o[t][4 * v + 2], R.o[t][4 * v + 3]};
-        if (h == 0) g.ml[row * slots + slot] = make_float2(R.m, R.l);
+        if (h == 0) g.ml[row * slots + slot] = make_float4(R.m, R.l, R.w, 0.f);
       }
     } else {
       float z = R.l * 0.f;
@@ -762,20 +772,25 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
           for (int v = 0; v < 4; ++v)
             write_out<DT>(a, at, 32 * t + 8 * v + 4 * h,
                           f32x4{R.o[t][4 * v] * inv, R.o[t][4 * v + 1] * inv, R.o[t][4 * v + 2] * inv, R.o[t][4 * v + 3] * inv});
-        if (a.lse && h == 0) a.lse[row] = (R.m + __builtin_amdgcn_logf(R.l)) * LN2;
+        if (a.lse && h == 0) a.lse[row] = (R.m + __builtin_amdgcn_logf(R.w)) * LN2;
       }
       redo = (uint32_t)__builtin_amdgcn_ballot_w64(bad && h == 0);
     }
   } else {
     // the waves' results of the same 32 rows are brought to one maximum and added through LDS
-    if (h == 0) sh.ml[wave][lane] = make_float2(R.m, R.l);
+    if (h == 0) sh.ml[wave][lane] = make_float4(R.m, R.l, R.w, 0.f);
     __syncthreads();
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, whole = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) m = fmaxf(m, sh.ml[w][lane & 31].x);
     const float from = m == -INFINITY ? 0.f : m;  // nothing seen
 #pragma unroll
-    for (int w = 0; w < 4; ++w) l = fmaf(__builtin_amdgcn_exp2f(sh.ml[w][lane & 31].x - from), sh.ml[w][lane & 31].y, l);
+    for (int w = 0; w < 4; ++w) {
+      const float4 x = sh.ml[w][lane & 31];
+      const float e = __builtin_amdgcn_exp2f(x.x - from);
+      l = fmaf(e, x.y, l);
+      whole = fmaf(e, x.z, whole);
+    }
     const float mine = __builtin_amdgcn_exp2f(R.m - from);
     if (sh.none) l = NAN;
     constexpr int CH = D / 4;  // 16-byte chunks of a row, swizzled by the row
@@ -789,7 +804,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
               f32x4{R.o[t][4 * v] * mine, R.o[t][4 * v + 1] * mine, R.o[t][4 * v + 2] * mine, R.o[t][4 * v + 3] * mine};
     }
     __syncthreads();
-    if (wave == 0 && h == 0) sh.ml[0][lane] = make_float2(m, l);
+    if (wave == 0 && h == 0) sh.ml[0][lane] = make_float4(m, l, whole, 0.f);
     __syncthreads();
     const int rows = std::min(32, nrows - row0);
     for (int i = threadIdx.x; i < rows * (DR / 4); i += 256) {
@@ -797,7 +812,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) o += *(const KU_LDS f32x4*)(lds + w * 32 * D * 4 + r * D * 4 + ((ch ^ (r & (CH - 1) & 31)) << 4));
-      const float2 x = sh.ml[0][r];
+      const float4 x = sh.ml[0][r];
       const RowAt where = at_row(row0 + r);
       const int64_t at = where.index(a);
       if (slots > 1) {
@@ -807,7 +822,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
         if (bad_sum(x.y) || x.y == 0.f || bad_sum(o[0]) || bad_sum(o[1]) || bad_sum(o[2]) || bad_sum(o[3])) atomicOr(&sh.redo, 1u << r);
         const float inv = 1.f / x.y;
         write_out<DT>(a, where, ch * 4, o * inv);
-        if (ch == 0 && a.lse) a.lse[at] = (x.x + __builtin_amdgcn_logf(x.y)) * LN2;
+        if (ch == 0 && a.lse) a.lse[at] = (x.x + __builtin_amdgcn_logf(x.z)) * LN2;
       }
     }
     if (slots == 1) {
@@ -824,7 +839,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   }
 }
 
-template <int DT, int D, int DR>
+template <int DT, int D, int DR, bool LSE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) sdpa_tiles_k(SdpaArgs g) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[Tile<DT, D, DR>::LDS];
   __shared__ SdpaShared sh;
@@ -833,9 +848,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   int unit;
   if (!unit_of(g.p, blockIdx.x, second, unit)) return;
   if (g.p.part[second].shared)
-    run_unit<DT, D, DR, true>(g, second, unit, lds, sh);
+    run_unit<DT, D, DR, LSE, true>(g, second, unit, lds, sh);
   else
-    run_unit<DT, D, DR, false>(g, second, unit, lds, sh);
+    run_unit<DT, D, DR, LSE, false>(g, second, unit, lds, sh);
 }
 
 // Joins the partial results of rows, eight slots a lane at a time: with SIDE slots of a row side by side
@@ -849,18 +864,18 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
   const int rows = a.batch * a.q_len * a.q_heads, row0 = ((int)blockIdx.x * 4 + wave) * ROWS, row = row0 + lane / (L * SIDE);
   const bool there = row < rows;
   const int n = there ? g.p.slots : 0;
-  const float2* ml = g.ml + (int64_t)row * g.p.slots;
+  const float4* ml = g.ml + (int64_t)row * g.p.slots;
   const f32x4* po = reinterpret_cast<const f32x4*>(g.po + (int64_t)row * g.p.slots * D) + ch;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, whole = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int i0 = 0; i0 < g.p.slots; i0 += U * SIDE) {
     f32x4 x[U];
-    float2 y[U];
+    float4 y[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int i = i0 + j * SIDE + sub;
       x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      y[j] = make_float2(-INFINITY, 0.f);
+      y[j] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
       if (i < n) {
         if (ch * 4 < a.dim) x[j] = po[i * L];
         y[j] = ml[i];
@@ -874,11 +889,13 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
     const float from = top == -INFINITY ? 0.f : top, old = __builtin_amdgcn_exp2f(m - from);
     m = top;
     l *= old;
+    whole *= old;
     acc *= old;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const float w = __builtin_amdgcn_exp2f(y[j].x - from);  // 0 for a slot that saw nothing
       l = fmaf(w, y[j].y, l);
+      whole = fmaf(w, y[j].z, whole);
       acc += x[j] * w;
     }
   }
@@ -886,6 +903,7 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
 #pragma unroll
   for (int o = L; o < L * SIDE; o <<= 1) {
     l += __shfl_xor(l, o, 64);
+    whole += __shfl_xor(whole, o, 64);
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] += __shfl_xor(acc[k], o, 64);
   }
@@ -896,7 +914,7 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
   constexpr uint64_t LANES = L * SIDE == 64 ? ~0ull : (1ull << (L * SIDE % 64)) - 1;
   if (there && (bad >> (lane / (L * SIDE) * (L * SIDE)) & LANES) == 0) {
     if (sub == 0) write_out<DT>(a, at, ch * 4, acc * (1.f / l));
-    if (a.lse && ch == 0 && sub == 0) a.lse[row] = (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (a.lse && ch == 0 && sub == 0) a.lse[row] = (m + __builtin_amdgcn_logf(whole)) * LN2;
   }
   if (bad)
     for (int i = 0; i < ROWS; ++i)
@@ -1009,7 +1027,10 @@ int64_t join_groups(int64_t rows, int slots, int d) {
 template <int DT, int D, int DR>
 void launch_d(const SdpaArgs& g, hipStream_t s) {
   const unsigned groups = (unsigned)tile_groups(g.p);
-  if (groups) hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR>), dim3(groups), dim3(256), 0, s, g);
+  if (groups && DT != GT_F32 && g.a.lse)
+    hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR, DT != GT_F32>), dim3(groups), dim3(256), 0, s, g);
+  else if (groups)
+    hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR, false>), dim3(groups), dim3(256), 0, s, g);
   const unsigned joins = (unsigned)join_groups((int64_t)g.a.batch * g.a.q_len * g.a.q_heads, g.p.slots, D);
   if (joins == 0) return;
   if (g.p.slots <= 8)
@@ -1096,7 +1117,7 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
 size_t sdpa_prefix_scratch_bytes(const KuHipSdpaPrefixArgs& a) {
   const SdpaPlan p = make_plan(a);
   if (a.batch == 0 || p.slots <= 1) return 0;
-  return a.batch * a.q_len * a.q_heads * (size_t)p.slots * (padded_dim(a.head_dim) * sizeof(float) + sizeof(float2));
+  return a.batch * a.q_len * a.q_heads * (size_t)p.slots * (padded_dim(a.head_dim) * sizeof(float) + sizeof(float4));
 }
 
 void launch_sdpa_prefix(const KuHipSdpaPrefixArgs& a, void* scratch, hipStream_t s) {
@@ -1106,7 +1127,7 @@ void launch_sdpa_prefix(const KuHipSdpaPrefixArgs& a, void* scratch, hipStream_t
   g.p = make_plan(a);
   const int d = padded_dim(a.head_dim);
   g.po = static_cast<float*>(scratch);
-  g.ml = reinterpret_cast<float2*>(g.po + a.batch * a.q_len * a.q_heads * (size_t)g.p.slots * d);
+  g.ml = reinterpret_cast<float4*>(g.po + a.batch * a.q_len * a.q_heads * (size_t)g.p.slots * d);
   switch (a.dtype) {
     case KU_BF16: launch_t<GT_BF16>(g, d, s); break;
     case KU_F16: launch_t<GT_F16>(g, d, s); break;

@@ -1,0 +1,79 @@
+"""How many bits ku_hip_sdpa_prefix keeps of its probabilities: keys whose probabilities round the same way."""
+import numpy as np
+import pytest
+
+from decode_ref import narrow, widen
+from kurumi_amd import DType
+from test_gpu_sdpa_prefix import Case
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {DType.BF16: 2.0 ** -8, DType.F16: 2.0 ** -11}  # of a value of 16 bits, relative to it
+
+# batch, q_len, q_heads, kv_heads: a few rows, whose waves deal the keys; rows of many sequences in tiles of 128;
+# rows of one sequence that fill such tiles
+ROWS = [(1, 1, 1, 1), (70, 1, 1, 1), (1, 128, 1, 1)]
+
+
+def two_levels(dt, rows, d, n, own, p, big):
+    """Keys of score 0 where `big`, of score ln p elsewhere (scale makes it so: q and k are 1 and -1 in one feature)."""
+    nb, nt, nh, kv = rows
+    c = Case(dt, nb, nt, nh, kv, d, 0, n if own else 0, lens=[n] * nb if own else None)
+    c.prefix, c.scale = 0 if own else n, float(np.float32(-np.log(p)))
+    c.q[:], one = 0, narrow(np.array([1.0, -1.0]), dt)
+    c.q[..., 0] = one[0]
+    keys = np.zeros((n, 1, d), c.q.dtype)
+    keys[~big, 0, 0] = one[1]
+    return c, keys, np.where(big, 0.0, 1.0)[:, None, None].repeat(d, 2)
+
+
+def place(c, keys, values, own):
+    if own:
+        for b in range(c.dims[0]):
+            at = b * c.seq_rows
+            c.k[at : at + len(keys)], c.v[at : at + len(keys)] = keys, narrow(values, c.dt)
+    else:
+        c.pk, c.pv = keys, narrow(values, c.dt)
+
+
+@pytest.mark.parametrize("dt", [DType.BF16, DType.F16])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("own", [False, True], ids=["shared", "own"])
+@pytest.mark.parametrize("rows", ROWS, ids=lambda r: "x".join(map(str, r)))
+def test_probabilities_that_round_the_same_way_leave_no_bias(hip, dt, d, own, rows):
+    """All values 1, all keys but one in 32 at one probability, whose rounding is off by nearly half a step: a mean of
+    ones is one. Numerator and denominator add the same roundings in other orders, n of them at most, each
+    off by n u of the sum: 2 n u = 2^-15.4 together, under half of the step of 2^-8 or 2^-11 below 1, so the output is 1.
+    (A quotient of rounded and unrounded sums would be off by the rounding, nearly 2^-8 or 2^-11.)
+    The causal mask of several queries leaves the earlier ones fewer keys, of both kinds.
+    lse is of the unrounded sum: a probability is off by 8 u (its exponent's rounding, exp2), the sum by n u, its
+    logarithm's value by 4 u (|lse| + 1)."""
+    print(f"sdpa_prefix bias {dt.name} d {d} own {own} {rows}", flush=True)
+    n = 192
+    p = 0.5 * (1 + HALF[dt] * 0.97)
+    big = np.arange(n) % 32 == 0
+    c, keys, values = two_levels(dt, rows, d, n, own, p, big)
+    place(c, keys, np.ones_like(values), own)
+    o, lse = c.run(hip)
+    np.testing.assert_array_equal(widen(o, dt), 1.0)
+    ps = np.where(big, 1.0, np.exp(-np.float64(c.scale)))
+    nt = rows[1]
+    want = np.array([np.log(ps[: n - (nt - 1 - t) if own else n].sum()) for t in range(nt)])[None, :, None]
+    assert (np.abs(lse - want) <= (n + 12) * U + 4 * U * (np.abs(want) + 1)).all()
+
+
+@pytest.mark.parametrize("dt", [DType.BF16, DType.F16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("nb,nt", [(1, 1), (70, 1), (2, 128)])
+def test_a_mean_of_ones_over_thousands_of_far_keys(hip, dt, d, nb, nt):
+    """4096 keys at 2^-21.05 of the largest, all values 1, on 256 kv heads of one set of keys (so that one unit meets them
+    all): the far keys are 2^-9.05 of the sum, numerator and denominator alike. Their roundings differ by 2 n u = 2^-11
+    of the sums at most, the output by its own half step: either sum without the far keys would be off by more."""
+    n, p = 4097, 2.0 ** -21.05
+    c, keys, values = two_levels(dt, (nb, nt, 256, 256), d, n, False, p, np.arange(n) == 0)
+    c.pk, c.pv = keys, narrow(np.ones_like(values), dt)
+    o, lse = c.run(hip, prefix_head_stride=0)
+    assert (np.abs(widen(o, dt) - 1) <= 2 * n * U + HALF[dt]).all()
+    want = np.log(1 + (n - 1) * np.exp(-np.float64(c.scale)))
+    # a far key is off by 8 u and its exponent's rounding, 4 u a power of two; few of them weigh much
+    assert (np.abs(lse - want) <= (n + 100) * U).all()
