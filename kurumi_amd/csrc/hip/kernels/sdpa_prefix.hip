@@ -148,6 +148,10 @@ template <int DT, int D, int DR, bool LSE>
 struct Rows {
   using T = Tile<DT, D, DR>;
   static constexpr bool WHOLE = LSE && DT != GT_F32;  // two sums
+  // Probabilities of f16 keys are formed 2^7 times as large (at most 2^15, with RESCALE): those below 2^-21 of the
+  // largest, not 2^-14, are rounded to a step of one size, 2^-32 of the largest being half of it. Without it 65536 keys
+  // far below one would leave up to 2^-9 of their values' size.
+  static constexpr float SHIFT = DT == GT_F16 ? 7.f : 0.f;
   u32x4 q[T::DS];
   f32x16 o[T::DTL];
   float m, l;  // m in powers of two, already times scale
@@ -213,6 +217,8 @@ struct Rows {
     l += r.l[0] + r.l[1];
     if constexpr (WHOLE) w += r.w[0] + r.w[1];
   }
+  // what a score in powers of two is brought to the exponent of a probability by; of nothing seen so far every score is -inf
+  __device__ __forceinline__ float exponent() const { return m == -INFINITY ? 0.f : SHIFT - m; }
   // keys from `left` on are not seen (left counts from the tile's first key)
   static __device__ __forceinline__ void mask(f32x16& s, int left) {
     const int lim = left - 4 * ((threadIdx.x & 63) >> 5);
@@ -274,7 +280,7 @@ struct Rows {
   // O^T += V^T P^T over 32 keys, with the probabilities' sums.
   __device__ __forceinline__ void weigh(const f32x16& s, float c, const KU_LDS unsigned char* V) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    const float em = m == -INFINITY ? 0.f : -m;  // nothing seen so far: every score is -inf
+    const float em = exponent();
     if constexpr (DT == GT_F32) {
       // 32 keys in a sum of their own, which then joins O: a chain of every key's products would have an
       // error that grows with the keys
@@ -638,7 +644,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
           if (active) {
             mask(sc, blk);
             R.rescale(sc, c);
-            const float em = R.m == -INFINITY ? 0.f : -R.m;
+            const float em = R.exponent();
             u32x4 p[4];
             typename Rows<DT, D, DR, LSE>::Sums rs;
             const int r = lane & 31;
@@ -736,6 +742,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   auto at_row = [&](int r) { return RowAt(g.p, pooled, b, kvh, r); };
   const bool there = row0 + (lane & 31) < nrows;
   const int slots = g.p.slots, slot = second ? g.p.part[0].splits + split : split;
+  R.m -= Rows<DT, D, DR, LSE>::SHIFT;  // what O and the sums are in units of
   R.l += other_half(R.l);
   R.w = Rows<DT, D, DR, LSE>::WHOLE ? R.w + other_half(R.w) : R.l;
   if (__builtin_amdgcn_ballot_w64(none) != 0 && lane == 0) atomicOr(&sh.none, 1u);

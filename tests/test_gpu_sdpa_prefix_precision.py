@@ -1,4 +1,5 @@
-"""How many bits ku_hip_sdpa_prefix keeps of its probabilities: keys whose probabilities round the same way."""
+"""How many bits ku_hip_sdpa_prefix keeps of its probabilities: keys whose probabilities round the same way,
+and very many keys far below the largest."""
 import numpy as np
 import pytest
 
@@ -77,3 +78,32 @@ def test_a_mean_of_ones_over_thousands_of_far_keys(hip, dt, d, nb, nt):
     want = np.log(1 + (n - 1) * np.exp(-np.float64(c.scale)))
     # a far key is off by 8 u and its exponent's rounding, 4 u a power of two; few of them weigh much
     assert (np.abs(lse - want) <= (n + 100) * U).all()
+
+
+@pytest.mark.parametrize("dt", [DType.BF16, DType.F16])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("own", [False, True], ids=["shared", "own"])
+@pytest.mark.parametrize("rows", ROWS, ids=lambda r: "x".join(map(str, r)))
+@pytest.mark.parametrize("power", [-18.3, -22.5, -25.5])
+def test_keys_far_below_the_largest_still_count(hip, dt, d, own, rows, power):
+    """One key in 32 holds zeros and stands 2^18 to 2^25 above the others, which hold 30000: what they add up to is the
+    whole output. A probability is rounded to half a step, in f16 to 2^-32 of the largest at least (values
+    are held 2^7 times as large, with 2^-25 as the least half step), and is off by 4 u of its exponent before that;
+    the sums over n keys by n u each, the output by half a step."""
+    print(f"sdpa_prefix far below {dt.name} d {d} own {own} {rows} 2^{power}", flush=True)
+    n = 192
+    big = np.arange(n) % 32 == 0
+    c, keys, values = two_levels(dt, rows, d, n, own, 2.0 ** power, big)
+    value = widen(narrow(np.array([30000.0]), dt), dt)[0]
+    place(c, keys, values * value, own)
+    o, _ = c.run(hip)
+    p, nt = np.exp(-np.float64(c.scale)), rows[1]
+    for t in range(nt):
+        left = n - (nt - 1 - t) if own else n
+        small, large = int((~big[:left]).sum()), int(big[:left].sum())
+        want = small * p * value / (large + small * p)
+        tol = want * (HALF[dt] + 8 * U + 4 * U * abs(power) + 2 * n * U + HALF[dt])
+        if dt == DType.F16:
+            tol += small * 2.0 ** -32 * value / large + 2.0 ** -25
+        got = widen(o[:, t], dt)
+        assert (np.abs(got - want) <= tol).all(), (t, got.ravel()[:3], want, tol)
