@@ -143,11 +143,17 @@ struct Tile {
 //
 // Probabilities of 16-bit keys are rounded to 16 bits for the second product, and the output is divided by the sum
 // of the rounded ones: where many round the same way, a mean with unrounded ones below would be off by that rounding.
-// lse is of the unrounded sum, which is formed where it is asked for (LSE).
+// lse is of the unrounded sum, which is formed where it is asked for (LSE). Heads of up to 32 features hold a
+// probability as two 16-bit values with a product each, its rounding and the rounding of what that left, to 2^-17 of
+// itself in bf16 and 2^-22 in f16, and one unrounded sum: there the second product is a small part of a block.
+// Larger heads hold one value, off by half a step (the output's own rounding is another): with two, 64 sequences on
+// 8192 keys of 128 features would take 60 us for 50, 32 on 65536 100 for 80, 8 x 256 queries on 4096 of 64 78 for 67
+// (kernel times, with lse).
 template <int DT, int D, int DR, bool LSE>
 struct Rows {
   using T = Tile<DT, D, DR>;
-  static constexpr bool WHOLE = LSE && DT != GT_F32;  // two sums
+  static constexpr bool TWO = DT != GT_F32 && D == 32;         // two values a probability
+  static constexpr bool WHOLE = LSE && DT != GT_F32 && !TWO;  // two sums
   // Probabilities of f16 keys are formed 2^7 times as large (at most 2^15, with RESCALE): those below 2^-21 of the
   // largest, not 2^-14, are rounded to a step of one size, 2^-32 of the largest being half of it. Without it 65536 keys
   // far below one would leave up to 2^-9 of their values' size.
@@ -205,11 +211,16 @@ struct Rows {
   // Sums of a block's probabilities of 16 bits, in two chains.
   struct Sums {
     float l[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
-    // two probabilities as the product takes them
-    __device__ __forceinline__ uint32_t add(int i, float p0, float p1) {
+    // two probabilities as the product takes them, `lo` what their rounding left
+    __device__ __forceinline__ uint32_t add(int i, float p0, float p1, uint32_t& lo) {
       const uint32_t pp = pack2<DT>(p0, p1);
-      l[i] = sum2<DT>(pp, l[i]);
-      if constexpr (WHOLE) w[i] += p0 + p1;
+      if constexpr (TWO) {
+        lo = pack2<DT>(p0 - lower<DT>(pp), p1 - upper<DT>(pp));
+        l[i] += p0 + p1;
+      } else {
+        l[i] = sum2<DT>(pp, l[i]);
+        if constexpr (WHOLE) w[i] += p0 + p1;
+      }
       return pp;
     }
   };
@@ -251,8 +262,9 @@ struct Rows {
   // V^T fragments by transposing reads: in each 16-lane group input lane 4 k' + j points at key row k',
   // dims 4 j.. + 3, and output lane i receives keys 0..3 of dim i; two of them fetch the keys that the
   // probability registers hold, 16 s + 4 h + 0..3 and those + 8.
+  // `lo`: the second values of the probabilities, where there are two.
   template <int STEPS>
-  __device__ __forceinline__ void product(const u32x4 (&p)[STEPS], const KU_LDS unsigned char* V) {
+  __device__ __forceinline__ void product(const u32x4 (&p)[STEPS], const u32x4 (&lo)[STEPS], const KU_LDS unsigned char* V) {
     const int lane = threadIdx.x & 63, h = lane >> 5, g = lane >> 4, c16 = lane & 15;
     auto read = [&](int st, u32x4 (&f)[T::DTL]) {
 #pragma unroll
@@ -274,7 +286,10 @@ struct Rows {
     for (int st = 0; st < STEPS; ++st) {
       if (st + 1 < STEPS) read(st + 1, f[(st + 1) & 1]);
 #pragma unroll
-      for (int t = 0; t < T::DTL; ++t) mfma_step<DT>(f[st & 1][t], p[st], o[t]);
+      for (int t = 0; t < T::DTL; ++t) {
+        mfma_step<DT>(f[st & 1][t], p[st], o[t]);
+        if constexpr (TWO) mfma_step<DT>(f[st & 1][t], lo[st], o[t]);
+      }
     }
   }
   // O^T += V^T P^T over 32 keys, with the probabilities' sums.
@@ -304,16 +319,18 @@ struct Rows {
         for (int v = 0; v < 16; ++v) o[t][v] += sum[v];
       }
     } else {
-      u32x4 p[2];
+      u32x4 p[2], lo[2];
       Sums r;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * i], c, em));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], c, em));
-        p[i >> 2][i & 3] = r.add(i & 1, p0, p1);
+        uint32_t rest = 0;
+        p[i >> 2][i & 3] = r.add(i & 1, p0, p1, rest);
+        lo[i >> 2][i & 3] = rest;
       }
       join(r);
-      product(p, V);
+      product(p, lo, V);
     }
   }
 };
@@ -645,7 +662,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
             mask(sc, blk);
             R.rescale(sc, c);
             const float em = R.exponent();
-            u32x4 p[4];
+            u32x4 p[4], lo[4];
             typename Rows<DT, D, DR, LSE>::Sums rs;
             const int r = lane & 31;
             const KU_LDS unsigned char* LK = kbuf(PAR ^ 1);
@@ -664,7 +681,9 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
                 const int te = i >> 3, v2 = i & 7;
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2], c, em));
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[te][2 * v2 + 1], c, em));
-                p[2 * te + (v2 >> 2)][v2 & 3] = rs.add(v2 & 1, p0, p1);
+                uint32_t rest = 0;
+                p[2 * te + (v2 >> 2)][v2 & 3] = rs.add(v2 & 1, p0, p1, rest);
+                lo[2 * te + (v2 >> 2)][v2 & 3] = rest;
               }
               if (m < 2) sn[m & 1] = f32x16{};
               mfma_step<DT>(kf[m % 3], R.q[m >> 1], sn[m & 1]);
@@ -672,7 +691,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
             }
             __builtin_amdgcn_s_setprio(0);
             R.join(rs);
-            R.product(p, vbuf(PAR));
+            R.product(p, lo, vbuf(PAR));
           }
           vm_wait<0>();
           __syncthreads();
@@ -1034,8 +1053,8 @@ int64_t join_groups(int64_t rows, int slots, int d) {
 template <int DT, int D, int DR>
 void launch_d(const SdpaArgs& g, hipStream_t s) {
   const unsigned groups = (unsigned)tile_groups(g.p);
-  if (groups && DT != GT_F32 && g.a.lse)
-    hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR, DT != GT_F32>), dim3(groups), dim3(256), 0, s, g);
+  if (groups && g.a.lse)
+    hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR, Rows<DT, D, DR, true>::WHOLE>), dim3(groups), dim3(256), 0, s, g);
   else if (groups)
     hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR, false>), dim3(groups), dim3(256), 0, s, g);
   const unsigned joins = (unsigned)join_groups((int64_t)g.a.batch * g.a.q_len * g.a.q_heads, g.p.slots, D);

@@ -1,5 +1,5 @@
 """How many bits ku_hip_sdpa_prefix keeps of its probabilities: keys whose probabilities round the same way,
-and very many keys far below the largest."""
+very many keys far below the largest, and heads of up to 32 features."""
 import numpy as np
 import pytest
 
@@ -10,6 +10,7 @@ from test_gpu_sdpa_prefix import Case
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 HALF = {DType.BF16: 2.0 ** -8, DType.F16: 2.0 ** -11}  # of a value of 16 bits, relative to it
+STEP_BITS = {DType.BF16: 7, DType.F16: 10}             # a value in [1, 2) lies 2^-bits from its neighbours
 
 # batch, q_len, q_heads, kv_heads: a few rows, whose waves deal the keys; rows of many sequences in tiles of 128;
 # rows of one sequence that fill such tiles
@@ -44,7 +45,8 @@ def place(c, keys, values, own):
 def test_probabilities_that_round_the_same_way_leave_no_bias(hip, dt, d, own, rows):
     """All values 1, all keys but one in 32 at one probability, whose rounding is off by nearly half a step: a mean of
     ones is one. Numerator and denominator add the same roundings in other orders, n of them at most, each
-    off by n u of the sum: 2 n u = 2^-15.4 together, under half of the step of 2^-8 or 2^-11 below 1, so the output is 1.
+    off by n u of the sum: 2 n u = 2^-15.4 together, under half of the step of 2^-8 or 2^-11 below 1, so the output is 1
+    (heads of 32 hold a probability to 2^-16 and more and add it unrounded: the same).
     (A quotient of rounded and unrounded sums would be off by the rounding, nearly 2^-8 or 2^-11.)
     The causal mask of several queries leaves the earlier ones fewer keys, of both kinds.
     lse is of the unrounded sum: a probability is off by 8 u (its exponent's rounding, exp2), the sum by n u, its
@@ -107,3 +109,36 @@ def test_keys_far_below_the_largest_still_count(hip, dt, d, own, rows, power):
             tol += small * 2.0 ** -32 * value / large + 2.0 ** -25
         got = widen(o[:, t], dt)
         assert (np.abs(got - want) <= tol).all(), (t, got.ravel()[:3], want, tol)
+
+
+@pytest.mark.parametrize("dt", [DType.BF16, DType.F16])
+@pytest.mark.parametrize("d", [8, 32])
+@pytest.mark.parametrize("own", [False, True], ids=["shared", "own"])
+@pytest.mark.parametrize("rows", ROWS, ids=lambda r: "x".join(map(str, r)))
+def test_heads_of_32_hold_a_probability_as_two_values(hip, dt, d, own, rows):
+    """Two keys of which one holds zeros, a query's probabilities different from the next one's: the output is one
+    probability times a value. Two values of 16 bits hold a probability to the square of half a step (f16: to
+    2^-32 at least), which is a hundredth of the output's own half step or less."""
+    print(f"sdpa_prefix two values {dt.name} d {d} own {own} {rows}", flush=True)
+    rng = np.random.default_rng(d)
+    nb, nt, nh, kv = rows
+    for trial in range(4):
+        c = Case(dt, nb, nt, nh, kv, d, 0 if own else 2, 2 + nt - 1 if own else 0, lens=[2 + nt - 1] * nb if own else None)
+        c.scale = 1.0
+        c.q[:] = 0
+        c.q[..., 0] = narrow(rng.uniform(0.1, 2.0, c.q.shape[:3]), dt)
+        minus = narrow(np.array([-1.0]), dt)[0]
+        # own keys: the first two are seen by all queries; the later ones score -inf-like, -1000 times a query
+        keys, values = np.zeros((2 + nt - 1 if own else 2, kv, d), c.q.dtype), np.zeros((2 + nt - 1 if own else 2, kv, d))
+        keys[1, :, 0] = minus
+        keys[2:, :, 0] = narrow(np.array([-30000.0]), dt)[0]
+        values[1] = rng.uniform(1, 2, (kv, d))
+        place(c, keys, values, own)
+        o, _ = c.run(hip)
+        p = np.exp(-widen(c.q[..., 0], dt))[..., None]
+        v = widen(narrow(values[1, 0], dt), dt)
+        want = p * v / (1 + p)
+        step = 2.0 ** (np.floor(np.log2(want)) - STEP_BITS[dt])
+        extra = want * (HALF[dt] ** 2 + 40 * U) + (2.0 ** -32 * 2 if dt == DType.F16 else 0)
+        got = widen(o, dt)
+        assert (np.abs(got - want) <= step / 2 + extra).all(), np.abs(got - want).max()
