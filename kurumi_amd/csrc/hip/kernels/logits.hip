@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8
         if (i + e < n) in[j].e[e] = x[i + e];
     }
   }
-  int32_t len = 0, prompt = 0, e0 = 0, e1 = 0;
+  int32_t len = 0, prompt = 0;
+  uint32_t e0 = 0, e1 = 0;  // below 2^31, so a place a round further is below 2^32
   if (a.tokens) {
     len = a.lens ? clamped(a.lens[r], a.history) : a.history;
     prompt = a.prompt_lens ? clamped(a.prompt_lens[r], len) : 0;
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8
         }
       }
     }
-    for (int32_t e = e0 + tid; e < e1; e += kThreads) {
+    for (uint32_t e = e0 + tid; e < e1; e += kThreads) {
       const int at = place(e == e0 + tid ? bias_id : a.bias_ids[e]);
       if (at != CHUNK && (atomicOr(&count[at], kBiased) & kBiased)) repeats = 1;
     }
@@ -192,13 +193,13 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8
   __syncthreads();
   const bool again = repeats;
   if (again) {
-    for (int32_t e = e0; e < e1; ++e) {
+    for (uint32_t e = e0; e < e1; ++e) {
       const int at = place(a.bias_ids[e]);
       if (at != CHUNK && at % kThreads == tid) count[at] = __float_as_uint(__uint_as_float(count[at]) + a.bias_values[e]);
     }
     __syncthreads();
   }
-  for (int32_t e = e0 + tid; e < e1; e += kThreads) {
+  for (uint32_t e = e0 + tid; e < e1; e += kThreads) {
     const int at = place(e == e0 + tid ? bias_id : a.bias_ids[e]);
     if (at == CHUNK || (bits && !(bits[at / 8] >> (at & 7) & 1))) continue;
     const float v = __uint_as_float(count[at]);
