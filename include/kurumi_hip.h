@@ -278,7 +278,7 @@ size_t ku_hip_codegen(KuGraph *g, const KuNode *roots, size_t n, uint32_t compil
  *   aligned device pointers; k a multiple of 128.
  * Enqueued on `stream` (a hipStream_t; NULL = the backend's stream), asynchronously. Scratch (the
  * quantised activation, m*k bytes) is a workspace of the backend that grows on demand, so calls
- * on one backend must be ordered on one stream. Returns 0, or -1 with ku_last_error. */
+ * of it on one backend must be ordered on one stream. Returns 0, or -1 with ku_last_error. */
 int32_t ku_hip_linear_e4m3(const KuBackend *b, const void *x, uint32_t x_dtype, const uint8_t *wq, const float *sw,
                            void *y, uint32_t y_dtype, size_t m, size_t n, size_t k, void *stream);
 
@@ -385,8 +385,8 @@ int32_t ku_hip_rope(const KuBackend *b, const KuHipRopeArgs *args, void *stream)
  * are multiples of 16 bytes. scale is positive and finite.
  *
  * Partial results need ku_hip_sdpa_prefix_scratch(args) bytes (0: none; it depends on the sizes
- * only). scratch NULL: a workspace of the backend that grows on demand, so such calls on one backend
- * must be ordered on one stream, and a call under stream capture is refused if it needs any (the
+ * only). scratch NULL: a workspace of the backend for these calls alone that grows on demand, so such
+ * calls on one backend must be ordered on one stream, and a call under stream capture is refused if it needs any (the
  * recorded graph would outlive the workspace). Calls, or graphs, that may overlap need a scratch each. */
 typedef struct KuHipSdpaPrefixArgs {
   uint32_t size; /* sizeof(KuHipSdpaPrefixArgs) */

@@ -684,7 +684,7 @@ int32_t ku_hip_linear_e4m3(const KuBackend* b, const void* x, uint32_t x_dtype, 
     ctx.make_current();
     const ku::hipbk::GemmRoute route = ku::hipbk::linear_e4m3_route(a.m, a.n, a.k);
     const size_t need = ku::hipbk::linear_e4m3_scratch_bytes(a.m, a.n, a.k, route);
-    void* ws = b->b->workspace(need);
+    void* ws = b->b->workspace(ku::hipbk::HipBackend::Entry::LinearE4m3, need);
     try {
       ku::hipbk::linear_e4m3(a, route, ws, need, stream ? static_cast<hipStream_t>(stream) : ctx.stream());
     } catch (const std::runtime_error& e) {

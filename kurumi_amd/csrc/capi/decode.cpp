@@ -105,7 +105,7 @@ int32_t ku_hip_sdpa_prefix(const KuBackend* b, const KuHipSdpaPrefixArgs* args, 
           KU_HIP(hipStreamIsCapturing(s, &st));
           if (st != hipStreamCaptureStatusNone)
             throw std::runtime_error("a captured call needs its own scratch (ku_hip_sdpa_prefix_scratch bytes)");
-          scratch = b->b->workspace(need);
+          scratch = b->b->workspace(ku::hipbk::HipBackend::Entry::SdpaPrefix, need);
         }
         ku::hipbk::launch_sdpa_prefix(a, scratch, s);
       });

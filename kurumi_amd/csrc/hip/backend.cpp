@@ -16,10 +16,12 @@ HipBackend::HipBackend(int device) {
 }
 
 HipBackend::~HipBackend() {
-  if (ws_.ptr) {
-    (void)hipDeviceSynchronize();
-    ctx_->pool().release(ws_);
-  }
+  (void)hipSetDevice(ctx_->device());
+  for (DevBuf& ws : ws_)
+    if (ws.ptr) {
+      (void)hipDeviceSynchronize();
+      ctx_->pool().release(ws);
+    }
   plans_.clear();
   consts_.reset();
   ctx_.reset();
@@ -49,22 +51,23 @@ std::shared_ptr<Plan> HipBackend::plan_for(const Graph& g, const std::vector<Nod
   }
   std::shared_ptr<Plan> p(new_plan(g, roots).release());
   plans_built_++;
-  plans_.push_front(Entry{g.id(), g.size(), roots, fp, p});
+  plans_.push_front(Cached{g.id(), g.size(), roots, fp, p});
   while (plans_.size() > kMaxCachedPlans) plans_.pop_back();
   return p;
 }
 
-void* HipBackend::workspace(size_t bytes) {
-  if (ws_.ptr && ws_.bytes >= bytes) return ws_.ptr;
+void* HipBackend::workspace(Entry entry, size_t bytes) {
+  DevBuf& ws = ws_[static_cast<size_t>(entry)];
+  if (ws.ptr && ws.bytes >= bytes) return ws.ptr;
   ctx_->make_current();
-  if (ws_.ptr) {
+  if (ws.ptr) {
     // kernels of earlier calls (on whatever stream the caller gave) may still read the old one
     KU_HIP(hipDeviceSynchronize());
-    ctx_->pool().release(ws_);
-    ws_ = DevBuf{};
+    ctx_->pool().release(ws);
+    ws = DevBuf{};
   }
-  ws_ = ctx_->pool().alloc(bytes);
-  return ws_.ptr;
+  ws = ctx_->pool().alloc(bytes);
+  return ws.ptr;
 }
 
 void feed_plan(Plan& p, const Feeds& feeds) {

@@ -27,23 +27,25 @@ class HipBackend : public ku::Backend {
   size_t plans_built() const { return plans_built_; }
   std::unique_ptr<Plan> new_plan(const Graph& g, const std::vector<NodeId>& roots);
   Context& ctx() { return *ctx_; }
-  // Grow-only device workspace of the direct kernel entry points (ku_hip_linear_e4m3): at least
-  // `bytes`, reused by every call on this backend (calls must be ordered on one stream).
-  void* workspace(size_t bytes);
+  // Grow-only device workspace of a direct kernel entry point: at least `bytes`, reused by every call of
+  // that entry on this backend (which must be ordered on one stream). Each entry has its own, so calls of
+  // different entries may run at once.
+  enum class Entry { LinearE4m3, SdpaPrefix, Count };
+  void* workspace(Entry entry, size_t bytes);
   ConstCache& consts() { return *consts_; }
 
  private:
   std::unique_ptr<Context> ctx_;
   std::unique_ptr<ConstCache> consts_;
-  struct Entry {
+  struct Cached {
     uint64_t gid;
     size_t gsize;
     std::vector<NodeId> roots;
     Hash128 fp;
     std::shared_ptr<Plan> plan;
   };
-  std::list<Entry> plans_;  // most recent first
-  DevBuf ws_;
+  std::list<Cached> plans_;  // most recent first
+  DevBuf ws_[static_cast<size_t>(Entry::Count)];
   size_t plans_built_ = 0;
 };
 

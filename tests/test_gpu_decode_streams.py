@@ -1,0 +1,51 @@
+"""The calls on device buffers on several streams."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from decode_ref import dev
+from hipmem import DevBuf, check, hip as hiprt, synchronize
+from kurumi_amd import DType
+from kutest import f32_to_bf16_bits
+from test_gpu_linear_e4m3 import quantise_rows
+from test_gpu_sdpa_prefix import Case
+
+pytestmark = pytest.mark.gpu
+
+
+def test_attention_beside_a_linear_on_another_stream(hip):
+    """Each orders its own calls on one stream of its own: neither has the other's workspace. Every round
+    starts both, and either's results are those of a run by itself."""
+    streams = [C.c_void_p(), C.c_void_p()]
+    for s in streams:
+        check(hiprt().hipStreamCreate(C.byref(s)), "hipStreamCreate")
+    m, n, k = 2048, 2048, 4096
+    rng = np.random.default_rng(1)
+    x = dev(f32_to_bf16_bits(rng.standard_normal((m, k), np.float32)))
+    wq, sw = (dev(a) for a in quantise_rows(rng.standard_normal((n, k), np.float32)))
+    y = DevBuf(2 * m * n)
+    c = Case(DType.BF16, 20, 1, 16, 4, 128, 5000, 600, page=16)
+    args = c.args()
+
+    def linear(stream):
+        hip.linear_e4m3(x.ptr, DType.BF16, wq.ptr, sw.ptr, y.ptr, DType.BF16, m, n, k, stream)
+
+    def alone():
+        hip.sdpa_prefix(args)
+        synchronize()
+        linear(None)
+        return (*c.results(), y.numpy(np.uint16, (m, n)))
+
+    want = alone()
+    for turn in range(12):
+        print(f"turn {turn}", flush=True)
+        for _ in range(3):
+            hip.sdpa_prefix(args, streams[0].value)
+            linear(streams[1].value)
+            hip.sdpa_prefix(args, streams[0].value)
+        got = (*c.results(), y.numpy(np.uint16, (m, n)))
+        for a, b in zip(got, want):
+            np.testing.assert_array_equal(a, b)
+    for s in streams:
+        check(hiprt().hipStreamDestroy(s), "hipStreamDestroy")
