@@ -88,8 +88,12 @@ inline bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
 // work-groups of `threads` in one launch, whose threads are counted in 32 bits
 inline int64_t max_blocks(int threads) { return 0xffffffffll / threads; }
 
-inline void check_launch() {
-  const hipError_t e = hipGetLastError();
+// Launches a kernel of one block of arguments. What the launch itself returns decides: an error that an earlier call of
+// the thread left behind is neither taken for this launch's nor cleared.
+template <class Args>
+void launch(void (*kernel)(Args), dim3 grid, int threads, size_t lds, hipStream_t s, const Args& args) {
+  void* p[] = {const_cast<Args*>(&args)};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3((unsigned)threads), p, lds, s);
   if (e != hipSuccess) throw std::runtime_error(std::string("launch failed: ") + hipGetErrorString(e));
 }
 

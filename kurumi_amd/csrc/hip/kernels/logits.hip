@@ -223,9 +223,9 @@ void launch_o(LogitsDev& d, int64_t rows, hipStream_t s) {
   d.chunks = (uint32_t)((d.vocab + chunk - 1) / chunk);
   const dim3 grid((unsigned)(d.chunks * rows));
   if (large)
-    hipLaunchKernelGGL((logits_k<DT, T, OT, O, kLarge>), grid, dim3(kThreads), 0, s, d);
+    launch(logits_k<DT, T, OT, O, kLarge>, grid, kThreads, 0, s, d);
   else
-    hipLaunchKernelGGL((logits_k<DT, T, OT, O, kSmall>), grid, dim3(kThreads), 0, s, d);
+    launch(logits_k<DT, T, OT, O, kSmall>, grid, kThreads, 0, s, d);
 }
 template <int DT, class T>
 void launch_t(LogitsDev& d, uint32_t out, int64_t rows, hipStream_t s) {
@@ -301,7 +301,6 @@ void launch_logits_adjust(const KuHipLogitsArgs& a, hipStream_t s) {
     case KU_F16: launch_t<GT_F16, uint16_t>(d, a.out_dtype, (int64_t)a.rows, s); break;
     default: launch_t<GT_F32, float>(d, a.out_dtype, (int64_t)a.rows, s); break;
   }
-  check_launch();
 }
 
 }  // namespace ku::hipbk

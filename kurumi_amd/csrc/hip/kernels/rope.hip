@@ -197,9 +197,9 @@ RopePlan make_plan(const KuHipRopeArgs& a) {
 template <int DT, class T, int V>
 void launch_v(const RopePlan& p, bool half, hipStream_t s) {
   if (half)
-    hipLaunchKernelGGL((rope_k<DT, T, V, true>), p.grid, dim3(kThreads), p.lds, s, p.d);
+    launch(rope_k<DT, T, V, true>, p.grid, kThreads, p.lds, s, p.d);
   else
-    hipLaunchKernelGGL((rope_k<DT, T, V, false>), p.grid, dim3(kThreads), p.lds, s, p.d);
+    launch(rope_k<DT, T, V, false>, p.grid, kThreads, p.lds, s, p.d);
 }
 template <int DT, class T>
 void launch_t(const RopePlan& p, bool half, hipStream_t s) {
@@ -298,7 +298,6 @@ void launch_rope(const KuHipRopeArgs& a, hipStream_t s) {
     case KU_F16: launch_t<GT_F16, uint16_t>(p, half, s); break;
     default: launch_t<GT_F32, float>(p, half, s); break;
   }
-  check_launch();
 }
 
 }  // namespace ku::hipbk

@@ -1054,15 +1054,15 @@ template <int DT, int D, int DR>
 void launch_d(const SdpaArgs& g, hipStream_t s) {
   const unsigned groups = (unsigned)tile_groups(g.p);
   if (groups && g.a.lse)
-    hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR, Rows<DT, D, DR, true>::WHOLE>), dim3(groups), dim3(256), 0, s, g);
+    launch(sdpa_tiles_k<DT, D, DR, Rows<DT, D, DR, true>::WHOLE>, dim3(groups), 256, 0, s, g);
   else if (groups)
-    hipLaunchKernelGGL((sdpa_tiles_k<DT, D, DR, false>), dim3(groups), dim3(256), 0, s, g);
+    launch(sdpa_tiles_k<DT, D, DR, false>, dim3(groups), 256, 0, s, g);
   const unsigned joins = (unsigned)join_groups((int64_t)g.a.batch * g.a.q_len * g.a.q_heads, g.p.slots, D);
   if (joins == 0) return;
   if (g.p.slots <= 8)
-    hipLaunchKernelGGL((sdpa_join_k<DT, D, 1>), dim3(joins), dim3(256), 0, s, g);
+    launch(sdpa_join_k<DT, D, 1>, dim3(joins), 256, 0, s, g);
   else
-    hipLaunchKernelGGL((sdpa_join_k<DT, D, 256 / D>), dim3(joins), dim3(256), 0, s, g);
+    launch(sdpa_join_k<DT, D, 256 / D>, dim3(joins), 256, 0, s, g);
 }
 template <int DT>
 void launch_t(const SdpaArgs& g, int d, hipStream_t s) {
@@ -1159,7 +1159,6 @@ void launch_sdpa_prefix(const KuHipSdpaPrefixArgs& a, void* scratch, hipStream_t
     case KU_F16: launch_t<GT_F16>(g, d, s); break;
     default: launch_t<GT_F32>(g, d, s); break;
   }
-  check_launch();
 }
 
 }  // namespace ku::hipbk

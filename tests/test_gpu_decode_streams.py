@@ -4,6 +4,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import kurumi_amd as K
 from decode_ref import dev
 from hipmem import DevBuf, check, hip as hiprt, synchronize
 from kurumi_amd import DType
@@ -49,3 +50,32 @@ def test_attention_beside_a_linear_on_another_stream(hip):
             np.testing.assert_array_equal(a, b)
     for s in streams:
         check(hiprt().hipStreamDestroy(s), "hipStreamDestroy")
+
+
+def small_calls(hip):
+    """One small call of each kind, and what it writes."""
+    c = Case(DType.F32, 2, 1, 4, 2, 64, 300, 20)
+    args = c.args()
+    rows, vocab, d = 3, 500, 64
+    x, y = dev(np.ones((rows, vocab), np.float32)), dev(np.zeros((rows, vocab), np.float32))
+    logits = K.LogitsArgs(dtype=DType.F32, out_dtype=DType.F32, rows=rows, vocab=vocab, logits=x.ptr, logits_stride=vocab, out=y.ptr, out_stride=vocab)
+    q, qo, pos = dev(np.ones((rows, d), np.float32)), dev(np.zeros((rows, d), np.float32)), dev(np.zeros(rows, np.int32))
+    rope = K.RopeArgs(dtype=DType.F32, scale=1.0, tokens=rows, q_heads=1, head_dim=d, rot_dim=d, freqs=K.rope_freqs(d), positions=pos.ptr, q=q.ptr,
+                      q_token_stride=d, q_head_stride=d, q_out=qo.ptr, q_out_token_stride=d, q_out_head_stride=d)
+    keep = (x, q, pos)
+    return [(lambda: hip.rope(rope), lambda: qo.numpy(np.float32, (rows, d)), keep), (lambda: hip.sdpa_prefix(args), lambda: c.results()[0], keep),
+            (lambda: hip.logits_adjust(logits), lambda: y.numpy(np.float32, (rows, vocab)), keep)]
+
+
+def test_an_error_of_an_earlier_call_is_not_the_launchs(hip):
+    """A call that the runtime refused (a device that is none) leaves its error with the thread: the launches that
+    follow are none the worse, and the error is still there for the program to see."""
+    L = hiprt()
+    for call, result, _ in small_calls(hip):
+        call()  # what is loaded at a first use is there
+        want = result()
+        L.hipGetLastError()
+        assert L.hipSetDevice(1 << 20) != 0
+        call()
+        assert L.hipGetLastError() != 0
+        np.testing.assert_array_equal(result(), want)
