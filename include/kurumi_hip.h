@@ -302,10 +302,12 @@ int32_t ku_hip_linear_e4m3_noalloc(const void *x, uint32_t x_dtype, const uint8_
  *
  * Each call takes one block of arguments: clear it, set `size` to sizeof the struct and what the call
  * needs. Pointers are device memory of the backend's GPU unless said otherwise, strides are in
- * elements, dtypes are KU_F32, KU_BF16 or KU_F16. The call is enqueued on `stream` (a hipStream_t;
- * NULL = the backend's stream) asynchronously, and reads the block (and `freqs`) before it returns,
- * so both may be reused at once. It leaves the current device as it was. Returns 0, or -1 with
- * ku_last_error; a refused call has launched nothing. Values that only the device sees (positions,
+ * elements, dtypes are KU_F32, KU_BF16 or KU_F16. The call is enqueued on `stream` (a hipStream_t)
+ * asynchronously, after what that stream holds. NULL = the backend's stream, which does not wait for
+ * the null stream, nor the null stream for it; a program whose work is on the null stream passes
+ * hipStreamLegacy. The call reads the block (and `freqs`) before it returns, so both may be reused at
+ * once. It leaves the current device as it was. Returns 0, or -1 with ku_last_error; a refused call has
+ * launched nothing. Values that only the device sees (positions,
  * lengths, indices) are bounds-checked there as each field says; they never make a kernel read or
  * write outside the buffers that the block describes. All three may be captured into a hipGraph. */
 

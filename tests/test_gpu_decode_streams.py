@@ -52,6 +52,52 @@ def test_attention_beside_a_linear_on_another_stream(hip):
         check(hiprt().hipStreamDestroy(s), "hipStreamDestroy")
 
 
+NULL_STREAM = 1  # hipStreamLegacy: the null stream, which a handle of 0 does not name in these calls
+
+
+@pytest.mark.parametrize("call", ["rope", "sdpa_prefix", "logits_adjust"])
+def test_the_null_stream_by_its_handle(hip, call):
+    """A program whose work is on the null stream: long copies, then the inputs' true values, the call, and the copy of
+    its outputs, with no wait between them. (With no handle the call is on the backend's own stream and would
+    not wait.) Every round gives the results of a run that waits after each step."""
+    L = hiprt()
+    to_device = 3  # hipMemcpyDeviceToDevice
+    L.hipMemcpyAsync.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]
+    rng = np.random.default_rng(2)
+    rows, n = 64, 4096
+    good, other = (dev(rng.standard_normal((rows, n)).astype(np.float32)) for _ in range(2))
+    x, y, z = (DevBuf(4 * rows * n) for _ in range(3))
+    long_a, long_b = DevBuf(1 << 30), DevBuf(1 << 30)
+    d, heads = 64, n // 64
+    keep = [dev(np.arange(rows, dtype=np.int32)), K.rope_freqs(d), dev(rng.standard_normal((300, d)).astype(np.float32))]
+    if call == "rope":
+        args = K.RopeArgs(dtype=DType.F32, scale=1.0, tokens=rows, q_heads=heads, head_dim=d, rot_dim=d, freqs=keep[1], positions=keep[0].ptr, q=x.ptr,
+                          q_token_stride=n, q_head_stride=d, q_out=y.ptr, q_out_token_stride=n, q_out_head_stride=d)
+    elif call == "sdpa_prefix":
+        args = K.SdpaPrefixArgs(dtype=DType.F32, scale=0.125, batch=rows, q_len=1, q_heads=heads, kv_heads=1, head_dim=d, q=x.ptr, q_batch_stride=n,
+                                q_token_stride=n, q_head_stride=d, out=y.ptr, out_batch_stride=n, out_token_stride=n, out_head_stride=d, prefix_len=300,
+                                prefix_k=keep[2].ptr, prefix_v=keep[2].ptr, prefix_row_stride=d, prefix_head_stride=d)
+    else:
+        args = K.LogitsArgs(dtype=DType.F32, out_dtype=DType.F32, rows=rows, vocab=n, logits=x.ptr, logits_stride=n, out=y.ptr, out_stride=n)
+    run = getattr(hip, call)
+
+    def copy(dst, src, nbytes):
+        check(L.hipMemcpyAsync(dst.ptr, src.ptr, nbytes, to_device, None), "hipMemcpyAsync")
+
+    copy(x, good, 4 * rows * n)
+    synchronize()
+    run(args)
+    want = y.numpy(np.float32, (rows, n))
+    for _ in range(4):
+        copy(x, other, 4 * rows * n)
+        synchronize()
+        copy(long_a, long_b, 1 << 30)
+        copy(x, good, 4 * rows * n)
+        run(args, NULL_STREAM)
+        copy(z, y, 4 * rows * n)
+        np.testing.assert_array_equal(z.numpy(np.float32, (rows, n)), want)
+
+
 def small_calls(hip):
     """One small call of each kind, and what it writes."""
     c = Case(DType.F32, 2, 1, 4, 2, 64, 300, 20)
