@@ -15,6 +15,7 @@ own = False
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 WIDTH = {"f32": 4, "bf16": 2, "f16": 2}
 DEV = "cuda"
+NULL_STREAM = 1  # hipStreamLegacy: what names the null stream, torch's default one, to the library
 _backend = None
 
 
@@ -191,7 +192,8 @@ def _outputs(s):
 
 
 def _own(s):
-    """The library's calls on the same buffers; a program keeps the block of arguments with its buffers."""
+    """The library's calls on the same buffers, on torch's current stream (whose inputs they read and whose work reads
+    their outputs); a program keeps the block of arguments with its buffers."""
     global _backend
     import kurumi_amd as ku
 
@@ -234,7 +236,7 @@ def _own(s):
                 bias_ids=p(s.bias_ids), bias_values=p(s.bias_values), bias_offsets=p(s.bias_offsets), bias_count=s.bias_ids.numel(), mask=p(s.mask),
                 mask_rows=s.mask.shape[0], mask_stride=s.mask.stride(0), mask_index=p(s.mask_rows)))
     call, args = s.call
-    call(args)
+    call(args, torch.cuda.current_stream().cuda_stream or NULL_STREAM)
     return _outputs(s)
 
 
