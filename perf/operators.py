@@ -236,7 +236,8 @@ def _own(s):
                 bias_ids=p(s.bias_ids), bias_values=p(s.bias_values), bias_offsets=p(s.bias_offsets), bias_count=s.bias_ids.numel(), mask=p(s.mask),
                 mask_rows=s.mask.shape[0], mask_stride=s.mask.stride(0), mask_index=p(s.mask_rows)))
     call, args = s.call
-    call(args, torch.cuda.current_stream().cuda_stream or NULL_STREAM)
+    # the handle by itself: torch.cuda.current_stream() makes an object around it, for 2.8 us
+    call(args, torch._C._cuda_getCurrentRawStream(_outputs(s)[0].device.index) or NULL_STREAM)
     return _outputs(s)
 
 
