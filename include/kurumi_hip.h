@@ -338,8 +338,10 @@ int32_t ku_hip_rope_freqs(size_t rot_dim, double base, uint32_t scaling, double 
  * whose row is outside [0, out_rows) is not stored (a padded batch: -1); rows that no token names
  * keep what they hold. Rows of one call have to differ: of two tokens with one row, either's values
  * may stay. An output may be its input itself (same pointer and strides; k and v then without
- * rows), otherwise they may not overlap. Any strides and alignments; as many bytes are moved at a time,
- * up to 16, as heads, rot_dim / 2, strides and pointers are made of.
+ * rows); otherwise outputs share no byte with an input or with each other. Their runs of head_dim
+ * elements may lie between each other's, as in the rows of one projection. Any strides and
+ * alignments; as many bytes are moved at a time, up to 16, as heads, rot_dim / 2, strides and pointers
+ * are made of.
  * rot_dim is even, 0 to min(head_dim, 256). */
 typedef struct KuHipRopeArgs {
   uint32_t size; /* sizeof(KuHipRopeArgs) */
@@ -374,7 +376,7 @@ int32_t ku_hip_rope(const KuBackend *b, const KuHipRopeArgs *args, void *stream)
  * j < own_lens[b] - (q_len - 1 - t). q head h reads kv head h / (q_heads / kv_heads). The shared keys
  * and values are read once for the whole batch. A query that sees no key gets zeros. Only keys that a
  * query sees count: what other rows hold (infinities and NaN too) does not matter.
- *   q, out  [batch, q_len, q_heads, head_dim], out not overlapping q
+ *   q, out  [batch, q_len, q_heads, head_dim]
  *   lse     [batch, q_len, q_heads] contiguous f32, or NULL: ln sum_j exp(scale * q . key_j), -inf for
  *           a query that sees no key; outputs of several calls over parts of the keys join by it
  *   prefix_k, prefix_v [prefix_len, kv_heads, head_dim] (prefix_len may be 0)
@@ -383,8 +385,9 @@ int32_t ku_hip_rope(const KuBackend *b, const KuHipRopeArgs *args, void *stream)
  *           + j % page_size (page_size a power of two; keys of a page whose index is outside
  *           [0, own_rows / page_size) count as not there)
  *   own_lens [batch], each taken into [0, own_max]; own_max (0: no own keys) sizes the launch
- * k and v share their strides. head_dim is a multiple of 16 bytes, up to 128; pointers and strides
- * are multiples of 16 bytes. scale is positive and finite.
+ * out, lse and scratch share no byte with what is read (own_rows rows of a cache, whichever are seen) nor
+ * with each other. k and v share their strides. head_dim is a multiple of 16 bytes, up to 128; pointers
+ * and strides are multiples of 16 bytes. scale is positive and finite.
  *
  * Partial results need ku_hip_sdpa_prefix_scratch(args) bytes (0: none; it depends on the sizes
  * only). scratch NULL: a workspace of the backend for these calls alone that grows on demand, so such
@@ -436,7 +439,7 @@ size_t ku_hip_sdpa_prefix_scratch(const KuHipSdpaPrefixArgs *args);
  *   mask   [mask_rows, mask_stride words]: bit v % 32 of word v / 32 set = v is allowed. Row r goes by
  *          mask row mask_index[r] (mask_index NULL: r); an index outside [0, mask_rows) leaves the row
  *          unmasked. mask NULL: none.
- * out may be logits itself (same dtype and stride), otherwise they may not overlap. */
+ * out may be logits itself (same dtype and stride); otherwise it shares no byte with what is read. */
 typedef struct KuHipLogitsArgs {
   uint32_t size; /* sizeof(KuHipLogitsArgs) */
   uint32_t dtype, out_dtype;

@@ -4,7 +4,9 @@
 #pragma once
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -80,9 +82,68 @@ inline int64_t written_span(int64_t inner, std::initializer_list<Axis> axes, con
   return whole;
 }
 
-inline bool overlap(const void* p, int64_t np, const void* q, int64_t nq) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return a < b + (uintptr_t)nq && b < a + (uintptr_t)np;
+// A buffer as a call reads or writes it: contiguous runs of `inner` elements of `width` bytes along strided axes, which
+// span less than 2^61 bytes (span_of).
+struct Buffer {
+  const void* p = nullptr;
+  int64_t inner = 0;  // bytes
+  int64_t span = 0;   // bytes from the first to one past the last; 0: nothing
+  struct {
+    int64_t last, stride;  // steps, bytes
+  } axes[3];
+  int used = 0;
+
+  Buffer() = default;
+  Buffer(const void* at, int64_t run, std::initializer_list<Axis> along, size_t width) : p(at), inner(run * (int64_t)width), span(inner) {
+    for (const Axis& x : along) {
+      if (x.n == 0) p = nullptr;
+      if (x.n <= 1 || x.stride == 0) continue;
+      axes[used++] = {(int64_t)x.n - 1, x.stride * (int64_t)width};
+      span += axes[used - 1].last * axes[used - 1].stride;
+    }
+    if (!p) span = 0;
+  }
+};
+
+// Whether two buffers have a byte in common. Their runs' places differ by a sum of strides times steps of the axes, in
+// ranges: the steps are tried from the longest stride down, those that the shorter ones cannot make up for left
+// out, which leaves few of them where an axis' steps go past the axes inside it. Layouts that leave too many to
+// try count as sharing.
+inline bool share(const Buffer& a, const Buffer& b) {
+  const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+  if (a.span == 0 || b.span == 0 || apart >= a.span || -apart >= b.span) return false;
+  struct Term {
+    int64_t stride, lo, hi;  // bytes; steps
+  } t[6];
+  int n = 0;
+  for (const Buffer* x : {&a, &b})
+    for (int i = 0; i < x->used; ++i) {
+      int k = 0;
+      while (k < n && t[k].stride > x->axes[i].stride) ++k;
+      if (k == n || t[k].stride != x->axes[i].stride) {
+        for (int j = n++; j > k; --j) t[j] = t[j - 1];
+        t[k] = {x->axes[i].stride, 0, 0};
+      }
+      if (x == &a) t[k].lo -= x->axes[i].last;
+      else t[k].hi += x->axes[i].last;
+    }
+  int64_t lo[7] = {}, hi[7] = {};  // what the terms from k on can add
+  for (int k = n; k-- > 0;) {
+    lo[k] = lo[k + 1] + t[k].stride * t[k].lo;
+    hi[k] = hi[k + 1] + t[k].stride * t[k].hi;
+  }
+  const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  int tries = 20000;
+  auto meet = [&](auto& self, int k, int64_t at) -> bool {
+    if (k == n) return at > -b.inner && at < a.inner;
+    // steps from whose place the terms after this one can still bring the runs together
+    const int64_t first = std::max(t[k].lo, floor_div(-b.inner - at - hi[k + 1], t[k].stride) + 1),
+                  last = std::min(t[k].hi, -floor_div(-(a.inner - at - lo[k + 1]), t[k].stride) - 1);
+    for (int64_t i = first; i <= last; ++i)
+      if (--tries < 0 || self(self, k + 1, at + i * t[k].stride)) return true;
+    return false;
+  };
+  return meet(meet, 0, apart);
 }
 
 // work-groups of `threads` in one launch, whose threads are counted in 32 bits

@@ -247,9 +247,10 @@ void check_logits_adjust(const KuHipLogitsArgs& a) {
   require((__int128)((a.vocab + kThreads * kLarge - 1) / (kThreads * kLarge)) * a.rows <= max_blocks(kThreads), "too many rows of this vocab");
   require((a.logits && a.out) || a.rows == 0, "null logits or out");
   require(aligned_to(a.logits, (size_t)w) && aligned_to(a.out, (size_t)wo), "pointers must be aligned to their elements");
-  const int64_t ni = span_of((int64_t)a.vocab, {{a.rows, a.logits_stride}}, "logits") * w;
-  const int64_t no = written_span((int64_t)a.vocab, {{a.rows, a.out_stride}}, "out") * wo;
-  if (a.rows && overlap(a.logits, ni, a.out, no))
+  span_of((int64_t)a.vocab, {{a.rows, a.logits_stride}}, "logits");
+  written_span((int64_t)a.vocab, {{a.rows, a.out_stride}}, "out");
+  const Buffer out(a.out, (int64_t)a.vocab, {{a.rows, a.out_stride}}, wo);
+  if (share(out, Buffer(a.logits, (int64_t)a.vocab, {{a.rows, a.logits_stride}}, w)))
     require(a.logits == a.out && a.dtype == a.out_dtype && (a.rows == 1 || a.logits_stride == a.out_stride),
             "out overlaps logits without being the same");
   require(a.history <= kCount, "history is more than 2^30 - 1");
@@ -270,6 +271,13 @@ void check_logits_adjust(const KuHipLogitsArgs& a) {
                         (const void*)a.bias_values, (const void*)a.bias_offsets, (const void*)a.mask,
                         (const void*)a.mask_index})
     require(aligned_to(p, 4), "pointers must be aligned to their elements");
+  const auto flat = [](const void* p, size_t n) { return Buffer(p, (int64_t)n, {}, 4); };
+  for (const Buffer& x :
+       {Buffer(a.tokens, (int64_t)a.history, {{a.rows, a.tokens_stride}}, 4), flat(a.lens, a.rows), flat(a.prompt_lens, a.rows),
+        flat(a.repetition, a.rows), flat(a.presence, a.rows), flat(a.frequency, a.rows), flat(a.bias_ids, a.bias_count),
+        flat(a.bias_values, a.bias_count), flat(a.bias_count ? a.bias_offsets : nullptr, a.rows + 1),
+        Buffer(a.mask, (int64_t)(a.vocab + 31) / 32, {{a.mask_rows, a.mask_stride}}, 4), flat(a.mask ? a.mask_index : nullptr, a.rows)})
+    require(!share(out, x), "out overlaps an array that is read");
 }
 
 void launch_logits_adjust(const KuHipLogitsArgs& a, hipStream_t s) {

@@ -267,15 +267,20 @@ void check_rope(const KuHipRopeArgs& a) {
     require(a.out_rows <= 0x7fffffff, "too many cache rows");
     if (!a.rows) require(a.out_rows >= a.tokens, "out_rows is less than tokens, and there are no rows");
   }
+  Buffer ins[3], outs[3];
+  int sides = 0;
   auto side = [&](const void* in, int64_t it, int64_t ih, void* out, int64_t orow, int64_t oh, size_t heads,
                   size_t out_rows, bool by_row, const char* what) {
     if (!in) return;
     require(aligned_to(in, (size_t)w) && aligned_to(out, (size_t)w), "pointers must be aligned to their elements");
-    const int64_t ni = span_of(d, {{a.tokens, it}, {heads, ih}}, what) * w;
-    const int64_t no = written_span(d, {{out_rows, orow}, {heads, oh}}, what) * w;
-    if (a.tokens && overlap(in, ni, out, no))
-      require(in == out && it == orow && ih == oh && !by_row,
+    span_of(d, {{a.tokens, it}, {heads, ih}}, what);
+    written_span(d, {{out_rows, orow}, {heads, oh}}, what);
+    const Buffer x(in, d, {{a.tokens, it}, {heads, ih}}, w), y(out, d, {{by_row ? out_rows : a.tokens, orow}, {heads, oh}}, w);
+    if (share(x, y))
+      require(in == out && (a.tokens == 1 || it == orow) && (heads == 1 || ih == oh) && !by_row,
               "an output overlaps its input without being the same (for k and v: the same, and no rows)");
+    ins[sides] = x;
+    outs[sides++] = y;
   };
   side(a.q, a.q_token_stride, a.q_head_stride, a.q_out, a.q_out_token_stride, a.q_out_head_stride, a.q_heads, a.tokens,
        false, "q or q_out");
@@ -286,6 +291,13 @@ void check_rope(const KuHipRopeArgs& a) {
   if (a.tokens) {
     const dim3 grid = make_plan(a).grid;
     require((int64_t)grid.x * grid.y <= max_blocks(kThreads), "too many tokens for one launch");
+    const Buffer numbers[] = {{a.positions, (int64_t)a.tokens, {}, 4}, {a.rows, (int64_t)a.tokens, {}, 4}};
+    for (int i = 0; i < sides; ++i) {
+      for (int j = 0; j < sides; ++j)
+        require(i == j || !share(outs[i], ins[j]), "an output overlaps the input of another");
+      for (int j = 0; j < i; ++j) require(!share(outs[i], outs[j]), "two outputs overlap");
+      for (const Buffer& x : numbers) require(!share(outs[i], x), "an output overlaps positions or rows");
+    }
   }
 }
 

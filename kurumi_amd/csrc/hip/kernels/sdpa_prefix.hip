@@ -1102,12 +1102,14 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
   require(aligned_to(a.scratch, 16), "scratch must be 16-byte aligned");
   strides16({a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.out_batch_stride, a.out_token_stride,
              a.out_head_stride});
-  const int64_t nq = span_of(d, {{a.batch, a.q_batch_stride}, {a.q_len, a.q_token_stride}, {a.q_heads, a.q_head_stride}}, "q");
-  const int64_t no = written_span(
-      d, {{a.batch, a.out_batch_stride}, {a.q_len, a.out_token_stride}, {a.q_heads, a.out_head_stride}}, "out");
+  const std::initializer_list<Axis> q_axes = {{a.batch, a.q_batch_stride}, {a.q_len, a.q_token_stride}, {a.q_heads, a.q_head_stride}},
+                                    out_axes = {{a.batch, a.out_batch_stride}, {a.q_len, a.out_token_stride}, {a.q_heads, a.out_head_stride}};
+  span_of(d, q_axes, "q");
+  written_span(d, out_axes, "out");
+  const Buffer q(a.q, d, q_axes, w), out(a.out, d, out_axes, w);
   if (a.batch) {
     pointers16({a.q, a.out});
-    require(!overlap(a.q, nq * w, a.out, no * w), "out overlaps q");
+    require(!share(q, out), "out overlaps q");
   }
   if (a.prefix_len) {
     pointers16({a.prefix_k, a.prefix_v});
@@ -1137,6 +1139,25 @@ void check_sdpa_prefix(const KuHipSdpaPrefixArgs& a) {
     const SdpaPlan p = make_plan(a);
     require(tile_groups(p) <= max_blocks(256) && join_groups(a.batch * a.q_len * a.q_heads, p.slots, padded_dim(a.head_dim)) <= max_blocks(256),
             "more queries than one launch takes");
+    // what is written shares nothing with what is read, nor with each other
+    const auto flat = [](const void* p, size_t n, size_t bytes) { return Buffer(p, (int64_t)n, {}, bytes); };
+    const size_t own = a.own_max ? 1 : 0, prefix = a.prefix_len ? 1 : 0;
+    const auto keys = [&](const void* p, size_t there, size_t rows, int64_t row, int64_t head) {
+      return Buffer(there ? p : nullptr, d, {{rows, row}, {a.kv_heads, head}}, w);
+    };
+    const __int128 table = (__int128)a.batch * (__int128)a.pages_per_seq;
+    const Buffer read[] = {q,
+                           keys(a.prefix_k, prefix, a.prefix_len, a.prefix_row_stride, a.prefix_head_stride),
+                           keys(a.prefix_v, prefix, a.prefix_len, a.prefix_row_stride, a.prefix_head_stride),
+                           keys(a.own_k, own, a.own_rows, a.own_row_stride, a.own_head_stride),
+                           keys(a.own_v, own, a.own_rows, a.own_row_stride, a.own_head_stride),
+                           flat(own ? a.own_lens : nullptr, a.batch, 4),
+                           flat(own ? a.pages : nullptr, (size_t)std::min<__int128>(table, (__int128)1 << 58), 4)};
+    const Buffer written[] = {out, flat(a.lse, a.batch * a.q_len * a.q_heads, 4), flat(a.scratch, a.scratch ? sdpa_prefix_scratch_bytes(a) : 0, 1)};
+    for (const Buffer& y : written) {
+      for (const Buffer& x : read) require(!share(y, x), "out, lse or scratch overlaps an input");
+      for (const Buffer& x : written) require(&x >= &y || !share(y, x), "two of out, lse and scratch overlap");
+    }
   }
 }
 
