@@ -375,7 +375,9 @@ int32_t ku_hip_rope(const KuBackend *b, const KuHipRopeArgs *args, void *stream)
  * t sees: the q_len queries are the sequence's last q_len positions, so query t sees own key j when
  * j < own_lens[b] - (q_len - 1 - t). q head h reads kv head h / (q_heads / kv_heads). The shared keys
  * and values are read once for the whole batch. A query that sees no key gets zeros. Only keys that a
- * query sees count: what other rows hold (infinities and NaN too) does not matter.
+ * query sees count: what other rows hold (infinities and NaN too) does not matter. A query that sees an
+ * infinity or NaN, or shares a tile with one that does, is done by itself, key after key: such a call
+ * takes a hundred times as long and more.
  *   q, out  [batch, q_len, q_heads, head_dim]
  *   lse     [batch, q_len, q_heads] contiguous f32, or NULL: ln sum_j exp(scale * q . key_j), -inf for
  *           a query that sees no key; outputs of several calls over parts of the keys join by it

@@ -21,8 +21,8 @@
 //
 // Only rows that some query sees are ever loaded (places past the end repeat the last one), so what lies
 // behind them cannot matter. A query whose sums are not finite, or that saw nothing, is done again from
-// the definition by sdpa_one: an infinity or NaN in a value that another query of the tile sees, and a
-// page that is none, come out right that way.
+// the definition by sdpa_one: an infinity or NaN in a value that another query of the tile sees comes out right that way
+// (64 queries of 32 heads on 8192 keys with one such value: 6 ms). Keys whose page is none are masked in their tiles.
 //
 // What bounds it, 32 heads over 8 of 128 features, us of both kernels:
 //   1 query each of 32 sequences, 65536 shared keys, f16 (303 MB): 77, 3.9 TB/s; the loop alone runs at the
@@ -237,6 +237,13 @@ struct Rows {
     for (int v = 0; v < 16; ++v)
       if ((v >> 2) * 8 + (v & 3) >= lim) s[v] = -INFINITY;
   }
+  // keys whose bit is not set are not there
+  static __device__ __forceinline__ void mask_absent(f32x16& s, uint32_t present) {
+    const uint32_t mine = present >> (4 * ((threadIdx.x & 63) >> 5));
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+      if (!(mine >> ((v >> 2) * 8 + (v & 3)) & 1)) s[v] = -INFINITY;
+  }
   // the new maximum over NT tiles of scores, O and l brought to it
   template <int NT>
   __device__ __forceinline__ void rescale(const f32x16 (&s)[NT], float c) {
@@ -348,13 +355,20 @@ struct Keys {
   bool flat;             // rows one after another, 64 of them within 2 GiB: the DMA takes buffer offsets
   int held = -1;         // pages held .. held + 63 of the table lie in `page`, one a lane: the loop over
   int page = 0;          // the blocks then loads nothing that the compiler would wait for
-  bool none = false;     // a page that is none was met
+  bool none = false;     // a page that is none lay among those held so far
 
+  __device__ __forceinline__ bool there(int pg) const { return pg >= 0 && pg < npages; }
   // The pages of the keys from j0 on, one a lane.
   __device__ __forceinline__ void hold(int j0) {
     const int last = (n - 1) >> shift;
     held = j0 >> shift;
     page = table[held + (threadIdx.x & 63) < last ? held + (threadIdx.x & 63) : last];
+    none |= __builtin_amdgcn_ballot_w64(!there(page)) != 0;
+  }
+  // bit i: key j0 + i of 32 has a page
+  __device__ __forceinline__ uint32_t present(int j0) const {
+    const int j = j0 + (threadIdx.x & 31);
+    return (uint32_t)__builtin_amdgcn_ballot_w64(there(table[(j < n ? j : n - 1) >> shift]));
   }
   // Byte offsets of the rows that this wave's share (of WAVES) of KEYS keys from j0 on reads.
   template <int KEYS, int WAVES>
@@ -371,12 +385,18 @@ struct Keys {
       for (int i = 0; i < N; ++i) {
         int j = j0 + (i * WAVES + wave) * RPD + r;
         j = j < n ? j : n - 1;
-        int pg = __builtin_amdgcn_ds_bpermute(((j >> shift) - held) << 2, page);
-        if (pg < 0 || pg >= npages) {
-          none = true;
-          pg = 0;
+        int pg = __builtin_amdgcn_ds_bpermute(((j >> shift) - held) << 2, page), at = j & ((1 << shift) - 1);
+        if (none) {
+          // keys of a page that is none are masked; their values, which meet a probability of 0, are those of a
+          // key that there is: the first of a page held
+          const uint64_t some = __builtin_amdgcn_ballot_w64(there(page));
+          const int spare = some ? __builtin_amdgcn_readlane(page, __builtin_ctzll(some)) : 0;
+          if (!there(pg)) {
+            pg = spare;
+            at = 0;
+          }
         }
-        off[i] = (((int64_t)pg << shift) + (j & ((1 << shift) - 1))) * stride;
+        off[i] = (((int64_t)pg << shift) + at) * stride;
       }
     } else {
 #pragma unroll
@@ -537,7 +557,7 @@ __device__ __forceinline__ void touch_arguments() {
 // LDS of a work-group beside the tiles of keys.
 struct SdpaShared {
   float4 ml[4][32];
-  uint32_t redo, none;
+  uint32_t redo;
 };
 
 // One unit: a tile of rows against a split of its keys. SHARED: four waves of 32 rows share blocks of
@@ -577,11 +597,10 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   const int np = second ? 0 : (a.prefix + bk - 1) / bk, no = (own_n + bk - 1) / bk;
   int split_first, split_last;
   split_range(part.by_splits, np + no, split, split_first, split_last);
-  bool none = false;
   Rows<DT, D, DR, LSE> R;
   R.clear();
   R.limit = 0;
-  if (threadIdx.x == 0) sh.redo = sh.none = 0;
+  if (threadIdx.x == 0) sh.redo = 0;
   __syncthreads();
   // a few rows' own pages are asked for before Q: their loads return in order, and the first DMA needs them
   Keys<DT, D, DR> ahead;
@@ -621,9 +640,13 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
       constexpr std::true_type IsV{};
       // keys that are not there or not seen
       auto mask = [&](f32x16 (&s)[T::SB], int blk) {
-        if (blk * BK + BK > all)
+        if (blk * BK + BK > all) {
 #pragma unroll
           for (int t = 0; t < T::SB; ++t) R.mask(s[t], (seg ? R.limit : all) - blk * BK - 32 * t);
+          if (S.none)
+#pragma unroll
+            for (int t = 0; t < T::SB; ++t) R.mask_absent(s[t], S.present(blk * BK + 32 * t));
+        }
       };
       if constexpr (DT == GT_F32) {
         // a step of f32 products takes longer than a read of LDS or the softmax: nothing to interleave
@@ -737,7 +760,10 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
         f32x16 s[1];
         s[0] = R.scores(K);
         if (more) fetch_k(blk + 4);
-        if (blk * 32 + 32 > all) R.mask(s[0], (seg ? R.limit : all) - blk * 32);
+        if (blk * 32 + 32 > all) {
+          R.mask(s[0], (seg ? R.limit : all) - blk * 32);
+          if (S.none) R.mask_absent(s[0], S.present(blk * 32));
+        }
         R.rescale(s, c);
         if (more)
           vm_wait<N>();
@@ -748,7 +774,6 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
         if (more) fetch_v(blk + 4);
       }
     }
-    none |= S.none;
   }
 
   {
@@ -764,10 +789,8 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   R.m -= Rows<DT, D, DR, LSE>::SHIFT;  // what O and the sums are in units of
   R.l += other_half(R.l);
   R.w = Rows<DT, D, DR, LSE>::WHOLE ? R.w + other_half(R.w) : R.l;
-  if (__builtin_amdgcn_ballot_w64(none) != 0 && lane == 0) atomicOr(&sh.none, 1u);
   uint32_t redo = 0;  // rows of this wave that are done again
   __syncthreads();
-  if (sh.none) R.l = NAN;
   if constexpr (SHARED) {
     const RowAt at = at_row(there ? row0 + (lane & 31) : 0);
     const int64_t row = at.index(a);
@@ -818,7 +841,6 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
       whole = fmaf(e, x.z, whole);
     }
     const float mine = __builtin_amdgcn_exp2f(R.m - from);
-    if (sh.none) l = NAN;
     constexpr int CH = D / 4;  // 16-byte chunks of a row, swizzled by the row
     if (there) {
       KU_LDS unsigned char* o = lds + wave * 32 * D * 4 + (lane & 31) * D * 4;

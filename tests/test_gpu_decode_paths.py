@@ -163,3 +163,34 @@ def test_rope_in_place_with_several_units_a_thread(hip, dt):
     want, tol = rope(widen(x[:, :turned], dt).reshape(t, hq + hk, d), pos, list(freqs), d, K.ROPE_HALF)
     assert_within(widen(got[:, :turned], dt).reshape(want.shape), want, tol + rounding(want, dt), "q, k")
     np.testing.assert_array_equal(got[:, turned:], x[:, turned:])
+
+
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("garbage", [0.0, np.nan])
+@pytest.mark.parametrize("nb,nt,nh,kv,d,prefix,own,page", [
+    (3, 1, 8, 2, 128, 300, 90, 8), (2, 1, 4, 2, 64, 0, 700, 1), (40, 2, 8, 2, 96, 500, 60, 16),  # a few rows of a sequence
+    (2, 40, 4, 2, 64, 130, 200, 4),                                                            # tiles of 128 rows
+    (2, 128, 2, 1, 32, 0, 200, 4), (1, 128, 2, 2, 128, 70, 333, 1), (33, 128, 8, 8, 32, 20, 130, 8)],  # prefix and own keys in one pass
+    ids=lambda x: str(x))
+def test_keys_of_absent_pages_are_masked_like_others(hip, dt, garbage, nb, nt, nh, kv, d, prefix, own, page):
+    """The same bits as keys that score -inf in their place: the rows go through the same tiles (a row that is done by
+    itself, as one whose sums are not finite, has other roundings, and takes a hundred times as long). What the
+    cache's first page holds, or an unused one, does not matter."""
+    print(f"sdpa_prefix absent pages masked {dt.name} {nb}x{nt}x{nh}x{kv}x{d} prefix {prefix} own {own} pages of {page}", flush=True)
+    lens = [own - 7 * (b % 4) for b in range(nb)]
+    c = Case(dt, nb, nt, nh, kv, d, prefix, own, lens=lens, page=page)
+    c.q[..., 0] = narrow(np.abs(widen(c.q[..., 0], dt)) + 0.1, dt)
+    absent = [(0, 0), (0, 3), (nb - 1, 2), (nb - 1, (lens[-1] - 1) // page), (nb // 2, 1)]
+    keys, values, pages = c.k.copy(), c.v.copy(), c.pages.copy()
+    for b, i in absent:
+        at = int(pages[b, i]) * page
+        c.k[at : at + page, :, 0] = narrow(np.array([-np.inf], np.float32), dt)[0]
+    want = c.run(hip)
+    c.k, c.v = keys, values
+    for n, (b, i) in enumerate(absent):
+        at = int(pages[b, i]) * page
+        if garbage != 0:
+            c.v[at : at + page] = narrow(np.array([garbage], np.float32), dt)[0]
+        c.pages[b, i] = (-1, c.npages, 2 ** 31 - 1, -2 ** 31, c.npages + 5)[n]
+    for x, y in zip(c.run(hip), want):
+        np.testing.assert_array_equal(x, y)
