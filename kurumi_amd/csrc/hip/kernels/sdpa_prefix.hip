@@ -59,6 +59,15 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // The running maximum moves only when a block exceeds it by more than this (in powers of two), so most
 // blocks leave O alone; probabilities reach 2^8 at most before they are normalised.
 constexpr float RESCALE = 8.f;
+// Probabilities of f16 keys are formed 2^7 times as large (at most 2^15, with RESCALE): those below 2^-21 of the
+// largest, not 2^-14, are rounded to a step of one size, 2^-32 of the largest being half of it. Without it 65536 keys
+// far below one would leave up to 2^-9 of their values' size. All sums carry the factor; lse takes it out.
+template <int DT>
+constexpr float SHIFT = DT == GT_F16 ? 7.f : 0.f;
+template <int DT>
+__device__ __forceinline__ float lse_of(float m, float sum) {
+  return (m + __builtin_amdgcn_logf(sum * (DT == GT_F16 ? 0.0078125f : 1.f))) * LN2;
+}
 
 // Division by a number known at the launch: a product, and one correction.
 struct Div {
@@ -154,10 +163,6 @@ struct Rows {
   using T = Tile<DT, D, DR>;
   static constexpr bool TWO = DT != GT_F32 && D == 32;         // two values a probability
   static constexpr bool WHOLE = LSE && DT != GT_F32 && !TWO;  // two sums
-  // Probabilities of f16 keys are formed 2^7 times as large (at most 2^15, with RESCALE): those below 2^-21 of the
-  // largest, not 2^-14, are rounded to a step of one size, 2^-32 of the largest being half of it. Without it 65536 keys
-  // far below one would leave up to 2^-9 of their values' size.
-  static constexpr float SHIFT = DT == GT_F16 ? 7.f : 0.f;
   u32x4 q[T::DS];
   f32x16 o[T::DTL];
   float m, l;  // m in powers of two, already times scale
@@ -229,7 +234,7 @@ struct Rows {
     if constexpr (WHOLE) w += r.w[0] + r.w[1];
   }
   // what a score in powers of two is brought to the exponent of a probability by; of nothing seen so far every score is -inf
-  __device__ __forceinline__ float exponent() const { return m == -INFINITY ? 0.f : SHIFT - m; }
+  __device__ __forceinline__ float exponent() const { return m == -INFINITY ? 0.f : SHIFT<DT> - m; }
   // keys from `left` on are not seen (left counts from the tile's first key)
   static __device__ __forceinline__ void mask(f32x16& s, int left) {
     const int lim = left - 4 * ((threadIdx.x & 63) >> 5);
@@ -786,7 +791,6 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
   auto at_row = [&](int r) { return RowAt(g.p, pooled, b, kvh, r); };
   const bool there = row0 + (lane & 31) < nrows;
   const int slots = g.p.slots, slot = second ? g.p.part[0].splits + split : split;
-  R.m -= Rows<DT, D, DR, LSE>::SHIFT;  // what O and the sums are in units of
   R.l += other_half(R.l);
   R.w = Rows<DT, D, DR, LSE>::WHOLE ? R.w + other_half(R.w) : R.l;
   uint32_t redo = 0;  // rows of this wave that are done again
@@ -821,7 +825,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
           for (int v = 0; v < 4; ++v)
             write_out<DT>(a, at, 32 * t + 8 * v + 4 * h,
                           f32x4{R.o[t][4 * v] * inv, R.o[t][4 * v + 1] * inv, R.o[t][4 * v + 2] * inv, R.o[t][4 * v + 3] * inv});
-        if (a.lse && h == 0) a.lse[row] = (R.m + __builtin_amdgcn_logf(R.w)) * LN2;
+        if (a.lse && h == 0) a.lse[row] = lse_of<DT>(R.m, R.w);
       }
       redo = (uint32_t)__builtin_amdgcn_ballot_w64(bad && h == 0);
     }
@@ -870,7 +874,7 @@ __device__ __forceinline__ void run_unit(const SdpaArgs& g, bool second, int id,
         if (bad_sum(x.y) || x.y == 0.f || bad_sum(o[0]) || bad_sum(o[1]) || bad_sum(o[2]) || bad_sum(o[3])) atomicOr(&sh.redo, 1u << r);
         const float inv = 1.f / x.y;
         write_out<DT>(a, where, ch * 4, o * inv);
-        if (ch == 0 && a.lse) a.lse[at] = (x.x + __builtin_amdgcn_logf(x.z)) * LN2;
+        if (ch == 0 && a.lse) a.lse[at] = lse_of<DT>(x.x, x.z);
       }
     }
     if (slots == 1) {
@@ -962,7 +966,7 @@ __global__ void __launch_bounds__(256) sdpa_join_k(SdpaArgs g) {
   constexpr uint64_t LANES = L * SIDE == 64 ? ~0ull : (1ull << (L * SIDE % 64)) - 1;
   if (there && (bad >> (lane / (L * SIDE) * (L * SIDE)) & LANES) == 0) {
     if (sub == 0) write_out<DT>(a, at, ch * 4, acc * (1.f / l));
-    if (a.lse && ch == 0 && sub == 0) a.lse[row] = (m + __builtin_amdgcn_logf(whole)) * LN2;
+    if (a.lse && ch == 0 && sub == 0) a.lse[row] = lse_of<DT>(m, whole);
   }
   if (bad)
     for (int i = 0; i < ROWS; ++i)
