@@ -79,6 +79,15 @@ def test_full_tiles_of_infinite_scores(hip, dt):
     assert np.isnan(widen(o[0, up], dt)).all() and np.isposinf(l[0, up]).all() and np.isfinite(widen(o[0, ~up], dt)).all()
 
 
+@pytest.mark.parametrize("dt", FLOATS)
+@pytest.mark.parametrize("size", [(3, 1, 8, 2, 128, 500, 60), (70, 1, 4, 4, 64, 300, 40), (2, 128, 2, 1, 96, 100, 200), (5, 2, 4, 2, 32, 90, 20)], ids=str)
+def test_the_output_does_not_depend_on_lse(hip, dt, size):
+    """lse is of another sum than the output in 16 bits: asked for or not, the output has the same bits."""
+    c = Case(dt, *size)
+    with_lse, without = c.run(hip)[0], c.run(hip, lse=None)[0]
+    np.testing.assert_array_equal(with_lse, without)
+
+
 # ---- logits_adjust: chunks of 8192 logits, which take a row for every CU at least ----
 
 
