@@ -321,7 +321,8 @@ typedef enum { KU_ROPE_UNSCALED = 0, KU_ROPE_LINEAR, KU_ROPE_BASE, KU_ROPE_BY_PA
  *                    frequency, the slowest is divided by factor
  *   KU_ROPE_BY_PARTS pairs that turn at least `high` times over `trained_len` positions keep their
  *                    frequency, those that turn at most `low` times are divided by factor, and those
- *                    between are blended linearly in the number of turns
+ *                    between are blended linearly in the number of turns (not in the pair's index: a
+ *                    checkpoint whose ramp runs over the indices needs frequencies of its own)
  * `trained_len`, `low` and `high` count for KU_ROPE_BY_PARTS only. Returns 0, or -1 with
  * ku_last_error. Needs no GPU. */
 int32_t ku_hip_rope_freqs(size_t rot_dim, double base, uint32_t scaling, double factor, double trained_len, double low,
@@ -374,10 +375,11 @@ int32_t ku_hip_rope(const KuBackend *b, const KuHipRopeArgs *args, void *stream)
  * over the prefix_len shared keys and values and those of sequence b's own own_lens[b] ones that query
  * t sees: the q_len queries are the sequence's last q_len positions, so query t sees own key j when
  * j < own_lens[b] - (q_len - 1 - t). q head h reads kv head h / (q_heads / kv_heads). The shared keys
- * and values are read once for the whole batch. A query that sees no key gets zeros. Only keys that a
- * query sees count: what other rows hold (infinities and NaN too) does not matter. A query that sees an
- * infinity or NaN, or shares a tile with one that does, is done by itself, key after key: such a call
- * takes a hundred times as long and more.
+ * and values are read once for every 128 queries of a kv head, whichever sequences these are of (of one
+ * sequence, where its queries fill such tiles by themselves). A query that sees no key gets zeros. Only
+ * keys that a query sees count: what other rows hold (infinities and NaN too) does not matter. A query
+ * that sees an infinity or NaN, or shares a tile with one that does, is done by itself, key after key:
+ * such a call takes a hundred times as long and more.
  *   q, out  [batch, q_len, q_heads, head_dim]
  *   lse     [batch, q_len, q_heads] contiguous f32, or NULL: ln sum_j exp(scale * q . key_j), -inf for
  *           a query that sees no key; outputs of several calls over parts of the keys join by it
@@ -386,15 +388,20 @@ int32_t ku_hip_rope(const KuBackend *b, const KuHipRopeArgs *args, void *stream)
  *           or with `pages` [batch, pages_per_seq] row pages[b][j / page_size] * page_size
  *           + j % page_size (page_size a power of two; keys of a page whose index is outside
  *           [0, own_rows / page_size) count as not there)
- *   own_lens [batch], each taken into [0, own_max]; own_max (0: no own keys) sizes the launch
+ *   own_lens [batch], each taken into [0, own_max]; own_max (0: no own keys) sizes the launch, whose
+ *           split between prefix and own keys goes by it and not by the lengths: near the longest of
+ *           them is fastest
  * out, lse and scratch share no byte with what is read (own_rows rows of a cache, whichever are seen) nor
  * with each other. k and v share their strides. head_dim is a multiple of 16 bytes, up to 128; pointers
- * and strides are multiples of 16 bytes. scale is positive and finite.
+ * and strides are multiples of 16 bytes. scale is positive and finite. Sums are f32. KU_BF16 and KU_F16
+ * round a probability to their 16 bits for the product with the values (half a step; heads of up to 32
+ * features hold it as two such values; KU_F16 to 2^-32 of the largest at least), and the output once.
  *
  * Partial results need ku_hip_sdpa_prefix_scratch(args) bytes (0: none; it depends on the sizes
  * only). scratch NULL: a workspace of the backend for these calls alone that grows on demand, so such
- * calls on one backend must be ordered on one stream, and a call under stream capture is refused if it needs any (the
- * recorded graph would outlive the workspace). Calls, or graphs, that may overlap need a scratch each. */
+ * calls on one backend must be ordered on one stream, and a call under stream capture is refused if it
+ * needs any (the recorded graph would outlive the workspace). Calls, or graphs, that may overlap need a
+ * scratch each. */
 typedef struct KuHipSdpaPrefixArgs {
   uint32_t size; /* sizeof(KuHipSdpaPrefixArgs) */
   uint32_t dtype;
