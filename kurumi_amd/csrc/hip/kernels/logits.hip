@@ -7,7 +7,8 @@
 // A work-group takes a chunk of one row's vocabulary and counts, in LDS, the row's tokens that fall
 // into it: whole numbers, so the order of the atomics does not matter. Nothing the size of the
 // vocabulary is kept or cleared in memory; every logit is read once and written once, and the row's
-// tokens and biases are read again (from L2) by each of its chunks.
+// tokens and biases are read again by each of its chunks: neighbouring chunks run on different XCDs, so
+// that each of these fetches a row's tokens into its own L2.
 #include <hip/hip_runtime.h>
 
 #include "decode.h"
@@ -210,9 +211,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(8
 
 // Large chunks read a row's tokens fewer times, small ones spread few rows over the chip; they meet where
 // there is a large one for every CU. us, large / small: 50257 logits, bf16 to f32, 1000 tokens: 16 rows
-// 7.1 / 5.2, 32 rows (224 chunks) 7.2 / 7.1, 64 rows 9.5 / 10.4, 128 rows 14.0 / 17.1; 32000 logits, f16,
-// 32768 tokens: 16 rows 10.6 / 9.2, 32 rows 11.8 / 12.4; 4 rows of 50257 f32 7.0 / 4.4; 256 rows of 131072,
-// 4000 tokens: 54.4 / 90.7. Of large ones, 12 or 24 logits a thread or 256 threads: the same within 2 us.
+// 7.0 / 5.4, 32 rows (224 chunks) 7.4 / 7.0, 64 rows 9.8 / 10.6, 128 rows 14.4 / 17.1; 32000 logits, f16,
+// 32768 tokens: 16 rows 10.7 / 9.2, 32 rows 12.0 / 12.2; 4 rows of 50257 f32 6.7 / 4.6; 256 rows of 131072,
+// 4000 tokens: 56.5 / 88. Of large ones, 12 or 24 logits a thread or 256 threads: the same within 2 us.
 bool large_chunks(int64_t vocab, int64_t rows) {
   return (vocab + kThreads * kLarge - 1) / (kThreads * kLarge) * rows >= (int64_t)cu_count();
 }

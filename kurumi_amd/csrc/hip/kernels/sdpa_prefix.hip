@@ -4,7 +4,7 @@
 // over the shared prefix and the keys of sequence b that query t sees.
 //
 // The queries that read one kv head are the rows of a matrix product with its keys. Over the prefix
-// the rows of every sequence go through together ("pooled"): a key is read once for the whole batch,
+// the rows of every sequence go through together ("pooled"): a key is read once for each tile of them,
 // which is what makes it a matrix product and not a vector one. A sequence's own keys meet its own rows
 // only. Where one sequence fills whole tiles of rows by itself (many queries), its tiles walk the prefix
 // and then its own keys in one pass ("joint").
@@ -24,13 +24,14 @@
 // the definition by sdpa_one: an infinity or NaN in a value that another query of the tile sees comes out right that way
 // (64 queries of 32 heads on 8192 keys with one such value: 6 ms). Keys whose page is none are masked in their tiles.
 //
-// What bounds it, 32 heads over 8 of 128 features, us of both kernels:
-//   1 query each of 32 sequences, 65536 shared keys, f16 (303 MB): 77, 3.9 TB/s; the loop alone runs at the
+// What bounds it, 32 heads over 8 of 128 features, with lse, us of both kernels:
+//   1 query each of 32 sequences, 65536 shared keys, f16 (303 MB): 81, 3.7 TB/s; the loop alone runs at the
 //     rate of a copy (5 TB/s), the rest is a unit's start, its partial result and the join
 //   64 sequences of up to 1024 own keys in pages of 16 beside 8192 shared ones, bf16 (171 MB): 50, 3.4 TB/s;
 //     the own keys, which few work-groups read with little in flight at the end
-//   256 queries each of 8 sequences, 16 heads over 4 of 64, 4096 shared keys, bf16 (37 GFLOP): 61, 0.6 PFLOP/s;
+//   256 queries each of 8 sequences, 16 heads over 4 of 64, 4096 shared keys, bf16 (37 GFLOP): 65, 0.6 PFLOP/s;
 //     the vector units: over 64 features a score's exponential and sums take as long as its two products
+// The second sum, for lse, takes 2 to 3 us of each.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -502,8 +503,8 @@ __device__ __forceinline__ bool unit_of(const SdpaPlan& p, int i, bool& second, 
 
 // The sequence of a batch of up to 64 that unit position i of the own keys takes: the longest first, so that
 // the last work-groups to start are the shortest, and by turns over the XCDs, each of which has a run of
-// positions. 64 sequences of 16 to 1024 keys beside 8192 shared ones: 44.8 us, 49.4 in their own order; 32
-// sequences 26.3 and 28.2; 16 queries each of 32 sequences 34.3 and 39.1.
+// positions. 64 sequences of 16 to 1024 keys beside 8192 shared ones: 44.4 us, 48.4 in their own order; 32
+// sequences 27.4 and 27.6.
 __device__ __forceinline__ int longest_first(const SdpaDev& a, int i, int& len) {
   const int lane = threadIdx.x & 63, n = a.batch;
   const int g = n & 7 ? (n & 3 ? (n & 1 ? 1 : 2) : 4) : 8, period = n / g;
@@ -1024,8 +1025,9 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     if (keys == 0 || items == 0 || rows == 0) return;
     // Tiles of 128 rows read a key once where four tiles of 32 read it four times (from L2, and with every
     // wave's own DMA); tiles of 32 spread few rows' keys over all four waves. us of both kernels, 128 / 32
-    // rows, bf16, 32 heads over 8 of 128, 8192 shared keys: 48 rows 19.8 / 17.4, 96 rows 22.1 / 21.2, 128 rows
-    // 31.9 / 34.9; 65536 keys: 64 rows 71.6 / 72.7, 128 rows 79.3 / 112.
+    // rows, bf16, 32 heads over 8 of 128, 8192 shared keys: 48 rows 20.5 / 17.4, 96 rows 23.2 / 21.0, 128 rows
+    // 25.0 / 22.1; 65536 keys: 64 rows 69.0 / 68.4, 128 rows 75.0 / 106: what short prefixes lose is less than
+    // what long ones would.
     part.shared = rows > 64;
     part.tiles = (int)((rows + (part.shared ? 127 : 31)) / (part.shared ? 128 : 32));
     const int64_t bk = part.shared ? (a.dtype == KU_F32 ? 32 : 64) : 128, blocks = (keys + bk - 1) / bk;
@@ -1037,21 +1039,23 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
   };
   if (p.joint) {
     // two a CU, so that one's products meet the other's exponentials: 256 queries each of 4 sequences on 4096
-    // shared keys, 16 heads over 4 of 128, 50 us and 64 with one; of one sequence 25 and 27
+    // shared keys, 16 heads over 4 of 128, 63 us and 71 with one; of one sequence 33 and 32; of 8 sequences,
+    // heads of 64, 65 and 82
     cut(p.part[0], per_seq, nb * kv, (int64_t)(a.prefix_len + a.own_max), 2 * cu);
   } else {
     // A unit costs about 4 us before its first product and 3 to write its partial result, so more of them
-    // than CUs lose: the prefix alone 30 us with one a CU, 38 with two and 38 with one for two CUs (256 rows,
-    // 8192 keys), 79 / 93 / 110 (128 rows, 65536 keys). Beside own keys of half its length or more it leaves
-    // every other CU to them: 50 us, and 55 with one a CU (64 sequences of up to 1024 own keys), 31 and 37
-    // (32 sequences).
+    // than CUs lose: the prefix alone 29 us with one a CU, 37 with two and 36 with one for two CUs (256 rows,
+    // 8192 keys), 76 / 85 / 107 (128 rows, 65536 keys). Beside own keys of half its length or more it leaves
+    // every other CU to them: 49 us, and 55 with one a CU (64 sequences of up to 1024 own keys), 33 and 38
+    // (32 sequences). own_max stands for the lengths, which the host does not know: of 64 sequences of up to
+    // 64 keys the call takes 39 us with an own_max of 64 or 4096, the prefix alone 31.
     const bool beside = nb * (int64_t)a.own_max * 2 >= (int64_t)a.prefix_len;
     cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len, beside ? cu / 2 : cu);
     // Own keys: a unit a CU, but halves where each sequence would be one unit and every CU had at most one,
-    // unless the prefix outlasts them. us of the tiles with cu / 2 cu units wanted, bf16, 8192 shared and up to
-    // 1024 own keys: 4 sequences 13.0 / 13.0, 8 15.5 / 17.0, 16 19.7 / 20.0; halves 32 sequences 26.0, whole 29.9;
-    // 4 sequences of up to 8192 27.9 / 32.7, one 11.8 / 14.2; under 65536 shared keys (32 sequences) 71.3 / 73.0;
-    // quarters cost 64 sequences 50 where they take 43.5.
+    // unless the prefix outlasts them. us of the tiles with cu / 2 and cu units wanted, bf16, 8192 shared and up to
+    // 1024 own keys: 4 sequences 12.7 / 13.0, 8 15.2 / 15.2, 16 18.2 / 18.4; up to 8192 own keys: 4 sequences 36.4 /
+    // 27.4, one 15.0 / 15.2. Wholes, halves and quarters: 32 sequences 28.8 / 27.5 / 31.5, 64 sequences (which
+    // stay whole) 44.3 / 48.4 / 57.9.
     cut(p.part[1], per_seq, nb * kv, (int64_t)a.own_max, cu, beside);
   }
   p.slots = p.part[0].splits + p.part[1].splits;
@@ -1070,7 +1074,7 @@ int padded_dim(size_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 int64_t tile_groups(const SdpaPlan& p) {
   return 8 * (((int64_t)p.part[0].units + 7) / 8 + ((int64_t)p.part[1].units + 7) / 8);
 }
-// Few slots: several rows a wave (32768 rows of 64, two slots: 7.2 us, and 14 with a wave a row).
+// Few slots: several rows a wave (32768 rows of 64, two slots: 7.4 us, and 14 with a wave a row).
 int64_t join_groups(int64_t rows, int slots, int d) {
   const int64_t each = 4 * (slots <= 8 ? 256 / d : 1);
   return slots == 1 ? 0 : (rows + each - 1) / each;
