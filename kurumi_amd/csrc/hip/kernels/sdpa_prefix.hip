@@ -162,7 +162,7 @@ struct Tile {
 template <int DT, int D, int DR, bool LSE>
 struct Rows {
   using T = Tile<DT, D, DR>;
-  static constexpr bool TWO = DT != GT_F32 && D == 32;         // two values a probability
+  static constexpr bool TWO = DT != GT_F32 && D == 32;        // two values a probability
   static constexpr bool WHOLE = LSE && DT != GT_F32 && !TWO;  // two sums
   u32x4 q[T::DS];
   f32x16 o[T::DTL];
@@ -1047,8 +1047,8 @@ SdpaPlan make_plan(const KuHipSdpaPrefixArgs& a) {
     // than CUs lose: the prefix alone 29 us with one a CU, 37 with two and 36 with one for two CUs (256 rows,
     // 8192 keys), 76 / 85 / 107 (128 rows, 65536 keys). Beside own keys of half its length or more it leaves
     // every other CU to them: 49 us, and 55 with one a CU (64 sequences of up to 1024 own keys), 33 and 38
-    // (32 sequences). own_max stands for the lengths, which the host does not know: of 64 sequences of up to
-    // 64 keys the call takes 39 us with an own_max of 64 or 4096, the prefix alone 31.
+    // (32 sequences). own_max stands for the lengths, which the host does not know: with up to 16 own keys
+    // and an own_max of 16 / 4096 8 sequences take 16.1 / 16.4, 16 16.4 / 19.8, 32 24.3 / 25.6, 64 28.6 / 36.1.
     const bool beside = nb * (int64_t)a.own_max * 2 >= (int64_t)a.prefix_len;
     cut(p.part[0], nb * per_seq, kv, (int64_t)a.prefix_len, beside ? cu / 2 : cu);
     // Own keys: a unit a CU, but halves where each sequence would be one unit and every CU had at most one,
